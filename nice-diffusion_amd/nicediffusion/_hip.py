@@ -1,4 +1,5 @@
-"""ctypes binding of ``libnd_hip.so`` (C ABI declared in ``include/nd_hip.h``).
+"""ctypes binding of ``libnd_hip.so`` (C ABI declared in ``include/nd_hip.h``) and of ``libnd_block.so``, the transformer-block
+operators (``include/nd_block.h``).
 
 There is no CPU fallback: if the library is missing, cannot be loaded, or the device is not gfx950 the sampling
 path raises.  PyTorch is used only for device memory, streams and graph capture.
@@ -25,6 +26,9 @@ VAR_LEARNED_INTERP = 2
 COEF_COLS = 8
 STEP_NO_CLIP = 1
 STEP_PER_IMAGE = 2
+
+# flags of libnd_block.so (mirror include/nd_block.h)
+ROPE_INTERLEAVED = 1
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -136,6 +140,18 @@ _SPECIAL = {
 }
 EXPORTS = sorted(list(SIGNATURES) + list(_SPECIAL))
 
+# libnd_block.so: (argtypes, restype)
+_T3 = [_vp, _i64, _i64, _i64]       # a [batch, token, head, channel] tensor: pointer and its three element strides
+BLOCK_SIGNATURES = {
+    'nd_block_build_id': ([], ctypes.c_char_p),
+    'nd_block_last_error': ([], ctypes.c_char_p),
+    'nd_qk_norm_rope': (_T3 * 2 + [_vp, _vp, _vp, _vp, _i64] + _T3 * 2 + [_i] * 6 + [_f, _i, _i, _vp], _i),
+    'nd_qk_norm_rope_bwd': (_T3 * 2 + [_vp, _vp, _vp, _vp, _i64] + _T3 * 4 + [_vp, _vp, _vp] + [_i] * 6 + [_f, _i, _i, _vp], _i),
+    'nd_qk_norm_rope_bwd_workspace_floats': ([_i] * 5, _i64),
+}
+_BLOCK = None
+_BLOCK_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libnd_block.so')
+
 
 class NdHipError(RuntimeError):
     pass
@@ -177,6 +193,35 @@ def load():
                          'construction; set ND_ALLOW_ABLATION=1 to load it for a measurement'.format(_LIB_PATH, flags))
     _LIB = L
     return L
+
+
+def block_path():
+    return _BLOCK_PATH
+
+
+def load_block():
+    """Load (once) and return libnd_block.so; raises NdHipError if it is not built."""
+    global _BLOCK
+    if _BLOCK is None:
+        import torch  # noqa: F401  (first: see load())
+        if not os.path.exists(_BLOCK_PATH):
+            raise NdHipError('libnd_block.so not found at {} -- build it with `make -C nice-diffusion_amd`; there is no CPU fallback'
+                             .format(_BLOCK_PATH))
+        try:
+            L = ctypes.CDLL(_BLOCK_PATH)
+        except OSError as e:   # pragma: no cover
+            raise NdHipError('cannot load {}: {}'.format(_BLOCK_PATH, e))
+        for name, (argtypes, restype) in BLOCK_SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = argtypes, restype
+        _BLOCK = L
+    return _BLOCK
+
+
+def check_block(rc, what=''):
+    if rc != 0:
+        raise NdHipError('{} failed (rc={}): {}'.format(what or 'libnd_block call', rc,
+                                                        load_block().nd_block_last_error().decode('utf-8', 'replace')))
 
 
 def build_id():
