@@ -44,6 +44,28 @@ int nd_qk_norm_rope_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                         int D, int R, float eps, int flags, int dtype, nd_stream_t stream);
 int64_t nd_qk_norm_rope_bwd_workspace_floats(int B, int T, int Hq, int Hk, int D);
 
+/* ---- gated feed-forward block ----------------------------------------------------------------------------------------- */
+
+#define ND_ACT_SILU 0
+#define ND_ACT_GELU 1      /* a Phi(a), with the error function */
+#define ND_ACT_GELU_TANH 2 /* its tanh form */
+
+/* y = residual + (act(x w_in[:F]^T + b_in[:F]) * (x w_in[F:]^T + b_in[F:])) w_out^T + b_out
+ * x [M, C] (row stride ldx), w_in [2F, C], b_in [2F] or NULL, w_out [C, F], b_out [C] or NULL, residual [M, C] (ldr) or NULL,
+ * y [M, C] (ldy; may be the residual's memory).  C, F multiples of 8; rows and pointers 16-byte aligned.  h [M, F]: scratch,
+ * and what the backward pass reads; au [M, 2F]: the pre-activations for the backward pass, or NULL. */
+int nd_gated_ffn(const void* x, int64_t ldx, const void* w_in, const void* b_in, const void* w_out, const void* b_out, const void* residual,
+                 int64_t ldr, void* y, int64_t ldy, void* h, void* au, float* workspace, int M, int C, int F, int act, int dtype,
+                 nd_stream_t stream);
+int64_t nd_gated_ffn_workspace_floats(int M, int C, int F, int dtype); /* may be 0: workspace NULL */
+
+/* gradients of nd_gated_ffn (any of dx [M, C], dw_in, db_in, dw_out, db_out may be NULL; that of the residual is dy); dau
+ * [M, 2F] is scratch for the first three */
+int nd_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_in, const void* w_out, const void* au,
+                     const void* h, void* dx, void* dw_in, void* db_in, void* dw_out, void* db_out, void* dau, float* workspace, int M,
+                     int C, int F, int act, int dtype, nd_stream_t stream);
+int64_t nd_gated_ffn_bwd_workspace_floats(int M, int C, int F, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,397 @@
+// Gated feed-forward block, forward and backward:
+//   [a | u] = x w_in^T + b_in,   h = act(a) u,   y = residual + h w_out^T + b_out            (x [M, C], w_in [2F, C], w_out [C, F])
+//   dh = dy w_out;  da = dh u act'(a);  du = dh act(a);  dx = [da | du] w_in;
+//   dw_in = [da | du]^T x;  dw_out = dy^T h;  db_in, db_out: column sums of [da | du], dy
+//
+// Six matrix products on the engine of blk_gemm.h.  The first makes the gate and the up columns of the same f in one wave, so
+// activation and product happen on the fp32 accumulators; its backward twin (dh) applies the derivative the same way.  MFMA
+// bound for long inputs: 6 M C F operations forward, 12 backward.
+//
+// Roundings to bf16 besides the outputs: h (operand of the second product), a and u where a backward pass will want them
+// (they are what it reads instead of repeating the first product: 2/9 of its operations), da and du (operands of two
+// products).  Each is half a unit, 2^-9 relative; fp32 calls round nothing.
+#include "blk_gemm.h"
+
+namespace ndb {
+
+template <int ACT>
+__device__ __forceinline__ void act_and_slope(float a, float& f, float& df) {
+    if constexpr (ACT == ND_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-a));
+        f = a * s;
+        df = s * (1.f + a * (1.f - s));
+    } else if constexpr (ACT == ND_ACT_GELU) {
+        const float cdf = 0.5f * (1.f + erff(a * 0.70710678118654752f));
+        f = a * cdf;
+        df = cdf + a * 0.3989422804014327f * __expf(-0.5f * a * a);
+    } else {      // 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z)),  z = sqrt(2 / pi) (a + 0.044715 a^3)
+        const float z2 = 1.5957691216057308f * a * (1.f + 0.044715f * a * a);
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z2));
+        f = a * s;
+        df = s + a * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * a * a);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* p) {
+    float t[4];
+    load_vec<T, 4>(p, t);
+    return f32x4{t[0], t[1], t[2], t[3]};
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const f32x4& v) {
+    const float t[4] = {v[0], v[1], v[2], v[3]};
+    store_vec<T, 4>(p, t);
+}
+
+template <typename T, int ACT>
+struct EpiGate {          // h = act(a) u, and a | u where they are kept
+    static constexpr bool GATED = true;
+    const T* bias;
+    T* h;
+    T* au;
+    int F;
+    __device__ __forceinline__ void operator()(int m, int f, f32x4 a, f32x4 u) const {
+        if (bias) {
+            a += load4(bias + f);
+            u += load4(bias + F + f);
+        }
+        f32x4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float v, d;
+            act_and_slope<ACT>(a[e], v, d);
+            r[e] = v * u[e];
+        }
+        store4(h + (int64_t)m * F + f, r);
+        if (au) {
+            store4(au + (int64_t)m * 2 * F + f, a);
+            store4(au + (int64_t)m * 2 * F + F + f, u);
+        }
+    }
+};
+
+template <typename T, int ACT>
+struct EpiGateBwd {       // dh -> da | du
+    static constexpr bool GATED = false;
+    const T* au;
+    T* dau;
+    int F;
+    __device__ __forceinline__ void operator()(int m, int f, int, f32x4 dh) const {
+        const int64_t at = (int64_t)m * 2 * F + f;
+        const f32x4 a = load4(au + at), u = load4(au + at + F);
+        f32x4 da, du;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float v, d;
+            act_and_slope<ACT>(a[e], v, d);
+            da[e] = dh[e] * u[e] * d;
+            du[e] = dh[e] * v;
+        }
+        store4(dau + at, da);
+        store4(dau + at + F, du);
+    }
+};
+
+template <typename T>
+struct EpiOut {           // bias, residual, one rounding
+    static constexpr bool GATED = false;
+    const T* bias;
+    const T* res;
+    T* out;
+    int64_t ldr, ldo;
+    __device__ __forceinline__ void operator()(int m, int n, int, f32x4 v) const {
+        if (bias) v += load4(bias + n);
+        if (res) v += load4(res + m * ldr + n);
+        store4(out + m * ldo + n, v);
+    }
+};
+
+struct EpiPart {          // one split's fp32 partial
+    static constexpr bool GATED = false;
+    float* out;
+    int64_t ld, split;
+    __device__ __forceinline__ void operator()(int m, int n, int sp, f32x4 v) const {
+        *reinterpret_cast<f32x4*>(out + sp * split + m * ld + n) = v;
+    }
+};
+
+// the partials of a split product in split order, then the epilogue; 4 columns a thread
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_join_kernel(const float* part, int splits, int M, int N, const EpiOut<T> epi) {
+    const int64_t quads = (int64_t)M * (N / 4);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i / (N / 4)), n = (int)(i - (int64_t)m * (N / 4)) * 4;
+        const float* p = part + (int64_t)m * N + n;
+        f32x4 v = *reinterpret_cast<const f32x4*>(p);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(p + s * (int64_t)M * N);
+        epi(m, n, 0, v);
+    }
+}
+
+// column sums of src [M, N]: 8 columns a thread, 8 rows side by side a block; partial row per block, then the rows in order
+template <typename T>
+__global__ void __launch_bounds__(256) colsum_kernel(const T* src, int64_t ld, int M, int N, float* part) {
+    __shared__ float red[8][257];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, n = (blockIdx.x * 32 + cx) * 8;
+    float s[8] = {};
+    if (n < N) {
+#pragma unroll 4
+        for (int m = blockIdx.y * 8 + ry; m < M; m += gridDim.y * 8) {
+            float v[8];
+            load_vec<T, 8>(src + m * ld + n, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += v[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[ry][cx * 8 + e] = s[e];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < N) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) t += red[r][threadIdx.x];
+        part[(int64_t)blockIdx.y * N + c] = t;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) colsum_join_kernel(const float* part, int rows, int N, T* out) {
+    __shared__ float red[32][33];
+    const int n = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+    float t = 0.f;
+    if (n < N)
+        for (int r = lane; r < rows; r += 32) t += part[(int64_t)r * N + n];
+    red[lane][threadIdx.x & 31] = t;
+    __syncthreads();
+    if (lane == 0 && n < N) {
+        float u = 0.f;
+        for (int l = 0; l < 32; ++l) u += red[l][threadIdx.x & 31];
+        out[n] = (T)u;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ launch choices
+struct Plan {
+    int big;              // 256 x 256 tiles (else 128 x 128)
+    int splits, k_tiles;
+};
+
+// Time of a product in stages: rounds of workgroups x stages each.  A 256-tile stage takes a CU 2048 matrix cycles, a
+// 128-tile one 512, but two of them share the CU and its LDS, which they read twice as much per operation.
+static Plan plan_gemm(int64_t M, int64_t N, int64_t K, int es, bool gated, bool may_split) {
+    const int kt = 128 / es;
+    const int64_t stages = (K + kt - 1) / kt;
+    Plan best{};
+    double best_t = 1e300;
+    for (int big = 0; big < 2; ++big) {
+        const int tile = big ? 256 : 128;
+        const int64_t tiles = ((M + tile - 1) / tile) * ((N + (gated ? tile / 2 : tile) - 1) / (gated ? tile / 2 : tile));
+        const int slots = big ? 256 : 512;
+        for (int want = 1; want <= (may_split ? 64 : 1); want *= 2) {
+            const int64_t per = (stages + want - 1) / want;
+            const int64_t splits = (stages + per - 1) / per;
+            if (want > 1 && (per < 4 || splits * M * N > (1LL << 28))) break;
+            const int64_t rounds = (tiles * splits + slots - 1) / slots;
+            double t = (double)rounds * (per + 3) * (big ? 2048.0 : 1.25 * 1024.0);
+            // the join moves splits + 1 fp32 copies at ~2 KiB a cycle over the chip, and is a launch of its own
+            if (splits > 1) t += 5000.0 + (double)(splits + 1) * M * N * 4 / 2048.0;
+            if (t < best_t) {
+                best_t = t;
+                best = {big, (int)splits, (int)per};
+            }
+        }
+    }
+    return best;
+}
+
+template <typename T, int TI, bool XK, bool WK, class Epi>
+static int launch_gemm(const char* fn, const GemmSide<T>& x, const GemmSide<T>& w, int K, const Plan& pl, int gate, const Epi& epi, hipStream_t st) {
+    constexpr int tile = 64 * TI;
+    GemmArgs<T> a{};
+    a.x = x, a.w = w, a.K = K, a.k_tiles = pl.k_tiles, a.splits = pl.splits, a.gate_rows = gate;
+    a.tiles_m = (x.n + tile - 1) / tile;
+    const int per_n = gate ? tile / 2 : tile, cols = gate ? gate : w.n;
+    a.tiles_n = (cols + per_n - 1) / per_n;
+    const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n * pl.splits;
+    NDB_REQUIRE(blocks <= (1 << 24), fn, "too many tiles for one launch");
+    auto kern = gemm_kernel<T, TI, XK, WK, Epi>;
+    static bool attr_set[kMaxDevices] = {};
+    if (int rc = ensure_max_lds(reinterpret_cast<const void*>(kern), attr_set, fn)) return rc;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(GEMM_THREADS), gemm_lds_bytes<TI>(), st, a, epi);
+    return check_launch(fn);
+}
+
+template <typename T, bool XK, bool WK, class Epi>
+static int run_gemm(const char* fn, const GemmSide<T>& x, const GemmSide<T>& w, int K, const Plan& pl, int gate, const Epi& epi, hipStream_t st) {
+    return pl.big ? launch_gemm<T, 4, XK, WK>(fn, x, w, K, pl, gate, epi, st) : launch_gemm<T, 2, XK, WK>(fn, x, w, K, pl, gate, epi, st);
+}
+
+// a product whose contraction may be split: straight to the output, or partials and their join
+template <typename T, bool XK, bool WK>
+static int run_gemm_out(const char* fn, const GemmSide<T>& x, const GemmSide<T>& w, int K, float* ws, const EpiOut<T>& epi, hipStream_t st) {
+    const Plan pl = plan_gemm(x.n, w.n, K, sizeof(T), false, true);
+    if (pl.splits == 1) return run_gemm<T, XK, WK>(fn, x, w, K, pl, 0, epi, st);
+    NDB_REQUIRE(ws, fn, "workspace missing");
+    const EpiPart part{ws, w.n, (int64_t)x.n * w.n};
+    if (int rc = run_gemm<T, XK, WK>(fn, x, w, K, pl, 0, part, st)) return rc;
+    const int64_t quads = (int64_t)x.n * (w.n / 4);
+    const int64_t blocks = (quads + 255) / 256;
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, ws, pl.splits, x.n, w.n, epi);
+    return check_launch(fn);
+}
+
+static int64_t split_floats(int64_t M, int64_t N, int64_t K, int es) {
+    const Plan pl = plan_gemm(M, N, K, es, false, true);
+    return pl.splits > 1 ? pl.splits * M * N : 0;
+}
+
+static int colsum_blocks(int64_t M, int64_t N) {
+    const int64_t cols = (N + 255) / 256, rows = (M + 63) / 64;
+    int64_t b = (2048 + cols - 1) / cols;
+    if (b > rows) b = rows;
+    return (int)(b < 1 ? 1 : (b > 1024 ? 1024 : b));
+}
+
+template <typename T>
+static int run_colsum(const char* fn, const T* src, int64_t ld, int M, int N, float* ws, T* out, hipStream_t st) {
+    const int rb = colsum_blocks(M, N);
+    hipLaunchKernelGGL((colsum_kernel<T>), dim3((N + 255) / 256, rb), dim3(256), 0, st, src, ld, M, N, ws);
+    hipLaunchKernelGGL((colsum_join_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, ws, rb, N, out);
+    return check_launch(fn);
+}
+
+template <typename T>
+struct Ffn {
+    const T *x, *w_in, *b_in, *w_out, *b_out, *res;
+    T *y, *h, *au;
+    int64_t ldx, ldr, ldy;
+    float* ws;
+    int M, C, F;
+};
+
+template <typename T, int ACT>
+static int ffn_forward(const char* fn, const Ffn<T>& a, hipStream_t st) {
+    const Plan pl = plan_gemm(a.M, a.F, a.C, sizeof(T), true, false);
+    if (int rc = run_gemm<T, true, true>(fn, GemmSide<T>{a.x, a.ldx, a.M}, GemmSide<T>{a.w_in, a.C, 2 * a.F}, a.C, pl, a.F,
+                                         EpiGate<T, ACT>{a.b_in, a.h, a.au, a.F}, st))
+        return rc;
+    return run_gemm_out<T, true, true>(fn, GemmSide<T>{a.h, a.F, a.M}, GemmSide<T>{a.w_out, a.F, a.C}, a.F, a.ws,
+                                       EpiOut<T>{a.b_out, a.res, a.y, a.ldr, a.ldy}, st);
+}
+
+template <typename T>
+struct FfnBwd {
+    const T *dy, *x, *w_in, *w_out, *au, *h;
+    T *dx, *dw_in, *db_in, *dw_out, *db_out, *dau;
+    int64_t lddy, ldx;
+    float* ws;
+    int M, C, F;
+};
+
+template <typename T, int ACT>
+static int ffn_backward(const char* fn, const FfnBwd<T>& a, hipStream_t st) {
+    const int M = a.M, C = a.C, F = a.F;
+    if (a.dau) {
+        const Plan pl = plan_gemm(M, F, C, sizeof(T), false, false);
+        if (int rc = run_gemm<T, true, false>(fn, GemmSide<T>{a.dy, a.lddy, M}, GemmSide<T>{a.w_out, F, F}, C, pl, 0,
+                                              EpiGateBwd<T, ACT>{a.au, a.dau, F}, st))
+            return rc;
+    }
+    if (a.dx)
+        if (int rc = run_gemm_out<T, true, false>(fn, GemmSide<T>{a.dau, 2 * F, M}, GemmSide<T>{a.w_in, C, C}, 2 * F, a.ws,
+                                                  EpiOut<T>{nullptr, nullptr, a.dx, 0, C}, st))
+            return rc;
+    if (a.dw_in)
+        if (int rc = run_gemm_out<T, false, false>(fn, GemmSide<T>{a.dau, 2 * F, 2 * F}, GemmSide<T>{a.x, a.ldx, C}, M, a.ws,
+                                                   EpiOut<T>{nullptr, nullptr, a.dw_in, 0, C}, st))
+            return rc;
+    if (a.dw_out)
+        if (int rc = run_gemm_out<T, false, false>(fn, GemmSide<T>{a.dy, a.lddy, C}, GemmSide<T>{a.h, F, F}, M, a.ws,
+                                                   EpiOut<T>{nullptr, nullptr, a.dw_out, 0, F}, st))
+            return rc;
+    if (a.db_in)
+        if (int rc = run_colsum<T>(fn, a.dau, 2 * F, M, 2 * F, a.ws, a.db_in, st)) return rc;
+    if (a.db_out)
+        if (int rc = run_colsum<T>(fn, a.dy, a.lddy, M, C, a.ws, a.db_out, st)) return rc;
+    return ND_OK;
+}
+
+static int ffn_check(const char* fn, int M, int C, int F, int act, int dtype) {
+    NDB_REQUIRE(M > 0 && C > 0 && F > 0, fn, "sizes must be positive");
+    NDB_REQUIRE(C % 8 == 0 && F % 8 == 0, fn, "channels and hidden channels must be multiples of 8");
+    NDB_REQUIRE((int64_t)C * F <= (1LL << 28), fn, "weights of more than 2^28 elements");
+    NDB_REQUIRE(act >= ND_ACT_SILU && act <= ND_ACT_GELU_TANH, fn, "unknown activation");
+    NDB_REQUIRE(dtype == ND_DT_F32 || dtype == ND_DT_BF16, fn, "dtype must be ND_DT_F32 or ND_DT_BF16");
+    return ND_OK;
+}
+
+static bool row_ok(const void* p, int64_t ld, int cols, int es) { return !p || (aligned_to(p, 16) && ld * es % 16 == 0 && ld >= cols && ld <= (1 << 21)); }
+
+}  // namespace ndb
+
+using namespace ndb;
+
+extern "C" int64_t nd_gated_ffn_workspace_floats(int M, int C, int F, int dtype) {
+    if (M <= 0 || C <= 0 || F <= 0) return -1;
+    return split_floats(M, C, F, dtype == ND_DT_BF16 ? 2 : 4);
+}
+
+extern "C" int nd_gated_ffn(const void* x, int64_t ldx, const void* w_in, const void* b_in, const void* w_out, const void* b_out,
+                            const void* residual, int64_t ldr, void* y, int64_t ldy, void* h, void* au, float* workspace, int M, int C,
+                            int F, int act, int dtype, nd_stream_t stream) {
+    const char* fn = "nd_gated_ffn";
+    if (int rc = ffn_check(fn, M, C, F, act, dtype)) return rc;
+    const int es = dtype == ND_DT_BF16 ? 2 : 4;
+    NDB_REQUIRE(x && w_in && w_out && y && h, fn, "null pointer");
+    NDB_REQUIRE(row_ok(x, ldx, C, es) && row_ok(residual, ldr, C, es) && row_ok(y, ldy, C, es), fn, "rows must be 16-byte aligned and no shorter than C");
+    NDB_REQUIRE(aligned_to(w_in, 16) && aligned_to(w_out, 16) && aligned_to(b_in, 16) && aligned_to(b_out, 16) && aligned_to(h, 16) && aligned_to(au, 16), fn,
+                "pointers must be 16-byte aligned");
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    auto go = [&](auto tag) {
+        using T = decltype(tag);
+        const Ffn<T> a{static_cast<const T*>(x), static_cast<const T*>(w_in), static_cast<const T*>(b_in), static_cast<const T*>(w_out),
+                       static_cast<const T*>(b_out), static_cast<const T*>(residual), static_cast<T*>(y), static_cast<T*>(h), static_cast<T*>(au),
+                       ldx, ldr, ldy, workspace, M, C, F};
+        return act == ND_ACT_SILU ? ffn_forward<T, ND_ACT_SILU>(fn, a, st)
+                                  : (act == ND_ACT_GELU ? ffn_forward<T, ND_ACT_GELU>(fn, a, st) : ffn_forward<T, ND_ACT_GELU_TANH>(fn, a, st));
+    };
+    return dtype == ND_DT_BF16 ? go(__bf16{}) : go(float{});
+}
+
+extern "C" int64_t nd_gated_ffn_bwd_workspace_floats(int M, int C, int F, int dtype) {
+    if (M <= 0 || C <= 0 || F <= 0) return -1;
+    const int es = dtype == ND_DT_BF16 ? 2 : 4;
+    int64_t n = split_floats(M, C, 2LL * F, es);
+    const int64_t more[4] = {split_floats(2LL * F, C, M, es), split_floats(C, F, M, es), (int64_t)colsum_blocks(M, 2LL * F) * 2 * F,
+                             (int64_t)colsum_blocks(M, C) * C};
+    for (int64_t v : more) n = v > n ? v : n;
+    return n;
+}
+
+extern "C" int nd_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_in, const void* w_out,
+                                const void* au, const void* h, void* dx, void* dw_in, void* db_in, void* dw_out, void* db_out, void* dau,
+                                float* workspace, int M, int C, int F, int act, int dtype, nd_stream_t stream) {
+    const char* fn = "nd_gated_ffn_bwd";
+    if (int rc = ffn_check(fn, M, C, F, act, dtype)) return rc;
+    const int es = dtype == ND_DT_BF16 ? 2 : 4;
+    NDB_REQUIRE(dy && (!dw_out || h) && (!dw_in || x) && (!dx || w_in), fn, "null pointer");
+    NDB_REQUIRE(!(dx || dw_in || db_in) || (dau && au && w_out), fn, "dx, dw_in and db_in need au, w_out and the dau buffer");
+    NDB_REQUIRE(workspace, fn, "workspace missing");
+    NDB_REQUIRE(row_ok(dy, lddy, C, es) && row_ok(x, ldx, C, es), fn, "rows must be 16-byte aligned and no shorter than C");
+    for (const void* p : {w_in, w_out, au, h, (const void*)dx, (const void*)dw_in, (const void*)dw_out, (const void*)dau, (const void*)workspace})
+        NDB_REQUIRE(aligned_to(p, 16), fn, "pointers must be 16-byte aligned");
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    auto go = [&](auto tag) {
+        using T = decltype(tag);
+        const FfnBwd<T> a{static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const T*>(w_in), static_cast<const T*>(w_out),
+                          static_cast<const T*>(au), static_cast<const T*>(h), static_cast<T*>(dx), static_cast<T*>(dw_in),
+                          static_cast<T*>(db_in), static_cast<T*>(dw_out), static_cast<T*>(db_out), dx || dw_in || db_in ? static_cast<T*>(dau) : nullptr,
+                          lddy, ldx, workspace, M, C, F};
+        return act == ND_ACT_SILU ? ffn_backward<T, ND_ACT_SILU>(fn, a, st)
+                                  : (act == ND_ACT_GELU ? ffn_backward<T, ND_ACT_GELU>(fn, a, st) : ffn_backward<T, ND_ACT_GELU_TANH>(fn, a, st));
+    };
+    return dtype == ND_DT_BF16 ? go(__bf16{}) : go(float{});
+}

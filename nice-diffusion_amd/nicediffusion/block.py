@@ -210,3 +210,124 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
     if q.numel():
         _launch_qk(q, k, q_weight, k_weight, cos, sin, eps, interleaved, qo, ko)
     return qo, ko
+
+
+# ------------------------------------------------------------------------------------------------ gated feed-forward
+_ACTS = {'silu': _hip.ACT_SILU, 'gelu': _hip.ACT_GELU, 'gelu_tanh': _hip.ACT_GELU_TANH}
+
+
+def _matrix(t, cols):
+    """``t`` [..., cols] as 16-byte aligned rows [M, cols] (a copy only where it does not lie like that)."""
+    m = t.reshape(-1, cols)
+    if m.stride(1) != 1 or (m.shape[0] > 1 and not cols <= m.stride(0) <= 1 << 21) or m.stride(0) * m.element_size() % 16 or m.data_ptr() % 16:
+        m = m.contiguous() if not m.is_contiguous() else m.clone()
+    return m
+
+
+def _ld(m):
+    return m.shape[1] if m.shape[0] == 1 else m.stride(0)
+
+
+def _aligned(t):
+    """A contiguous parameter on a 16-byte boundary."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _floats(n, device):
+    return torch.empty(n, dtype=torch.float32, device=device) if n > 0 else None
+
+
+def _launch_ffn(x, w_in, b_in, w_out, b_out, res, act, keep):
+    M, C = x.shape
+    F = w_out.shape[1]
+    new = dict(dtype=x.dtype, device=x.device)
+    y, h = torch.empty(M, C, **new), torch.empty(M, F, **new)
+    au = torch.empty(M, 2 * F, **new) if keep else None
+    ws = _floats(_hip.load_block().nd_gated_ffn_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
+    _call('nd_gated_ffn', x.device, x.data_ptr(), _ld(x), w_in.data_ptr(), _hip.ptr(b_in), w_out.data_ptr(), _hip.ptr(b_out), _hip.ptr(res),
+          0 if res is None else _ld(res), y.data_ptr(), C, h.data_ptr(), _hip.ptr(au), _hip.ptr(ws), M, C, F, act, _DT[x.dtype])
+    return y, h, au
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, b_in, w_out, b_out, res, act):
+        C = x.shape[-1]
+        xm, wi, wo = _matrix(x, C), _aligned(w_in), _aligned(w_out)
+        rm = None if res is None else _matrix(res, C)
+        if xm.shape[0]:
+            y, h, au = _launch_ffn(xm, wi, _aligned(b_in), wo, _aligned(b_out), rm, act, True)
+        else:
+            y, h, au = xm.new_empty(0, C), None, None
+        ctx.save_for_backward(xm, wi, wo, h, au)
+        ctx.act, ctx.shape = act, x.shape
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w_in, w_out, h, au = ctx.saved_tensors
+        M, C = x.shape
+        F = w_out.shape[1]
+        need = ctx.needs_input_grad
+        new = dict(dtype=x.dtype, device=x.device)
+        dx = torch.empty(M, C, **new) if need[0] else None
+        dwi = torch.empty(2 * F, C, **new) if need[1] else None
+        dbi = torch.empty(2 * F, **new) if need[2] else None
+        dwo = torch.empty(C, F, **new) if need[3] else None
+        dbo = torch.empty(C, **new) if need[4] else None
+        if M:
+            if any(need[:5]):
+                g = _matrix(dy, C)
+                dau = torch.empty(M, 2 * F, **new) if any(need[:3]) else None
+                ws = _floats(_hip.load_block().nd_gated_ffn_bwd_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
+                _call('nd_gated_ffn_bwd', x.device, g.data_ptr(), _ld(g), x.data_ptr(), _ld(x), w_in.data_ptr(), w_out.data_ptr(), au.data_ptr(),
+                      h.data_ptr(), _hip.ptr(dx), _hip.ptr(dwi), _hip.ptr(dbi), _hip.ptr(dwo), _hip.ptr(dbo), _hip.ptr(dau), _hip.ptr(ws), M, C,
+                      F, ctx.act, _DT[x.dtype])
+        else:
+            for t in (dwi, dbi, dwo, dbo):
+                if t is not None:
+                    t.zero_()
+        return None if dx is None else dx.view(ctx.shape), dwi, dbi, dwo, dbo, dy if need[5] else None, None
+
+
+def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, residual=None, activation='silu'):
+    """``residual + (act(x Wg^T + bg) * (x Wu^T + bu)) w_out^T + b_out``: the block's gated feed-forward half.
+
+    x [..., C]; w_in [2F, C]: the gate's rows Wg, then the up projection's Wu; w_out [C, F]; b_in [2F], b_out [C], residual
+    (x's shape) or None.  C and F multiples of 8.  activation: 'silu', 'gelu' (error function) or 'gelu_tanh'.  Returns a new
+    contiguous tensor of x's shape.  In bfloat16 the hidden row is rounded once between the two products; a backward pass keeps
+    it and the pre-activations (3 F values a token)."""
+    if activation not in _ACTS:
+        raise ValueError('activation is {!r}, expected one of {}'.format(activation, sorted(_ACTS)))
+    if x.dim() < 1:
+        raise ValueError('x has no channel dimension')
+    C = x.shape[-1]
+    if w_in.dim() != 2 or w_in.shape[0] % 2:
+        raise ValueError('w_in has shape {}, expected [2 F, {}]'.format(tuple(w_in.shape), C))
+    F = w_in.shape[0] // 2
+    _shape(w_in, 'w_in', 2 * F, C)
+    _shape(w_out, 'w_out', C, F)
+    if C == 0 or F == 0 or C % 8 or F % 8:
+        raise ValueError('channels ({}) and hidden channels ({}) must be positive multiples of 8'.format(C, F))
+    if C * F > 1 << 28:
+        raise ValueError('weights of more than 2^28 elements')
+    if b_in is not None:
+        _shape(b_in, 'b_in', 2 * F)
+    if b_out is not None:
+        _shape(b_out, 'b_out', C)
+    if residual is not None:
+        _shape(residual, 'residual', *x.shape)
+    _check(('x', x), w_in=w_in, w_out=w_out, b_in=b_in, b_out=b_out, residual=residual)
+    if x.numel() // C >= 1 << 31:
+        raise ValueError('too many rows')
+    act = _ACTS[activation]
+    if _wants_grad(x, w_in, b_in, w_out, b_out, residual):
+        return _GatedFfn.apply(x, w_in, b_in, w_out, b_out, residual, act)
+    if x.numel() == 0:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    res = None if residual is None else _matrix(residual, C)
+    return _launch_ffn(_matrix(x, C), _aligned(w_in), _aligned(b_in), _aligned(w_out), _aligned(b_out), res, act, False)[0].view(x.shape)

@@ -165,3 +165,100 @@ def test_qk_norm_rope_empty_and_unaligned():
     # lanes hold other channels, so the row sum is taken in another order: a last-place difference at most
     assert rel(a, b.double()) <= 2 * half_ulp(BF)
     assert rel(a, qk_ref(q, None, None, None, 1e-6, False)) <= half_ulp(BF) + 1e-5
+
+
+# ------------------------------------------------------------------------------------------------ gated_feed_forward
+def ffn_ref(x, w_in, w_out, b_in, b_out, res, act):
+    F = w_out.shape[1]
+    a = x @ w_in.t()
+    if b_in is not None:
+        a = a + b_in
+    a, u = a[..., :F], a[..., F:]
+    if act == 'silu':
+        f = a * torch.sigmoid(a)
+    elif act == 'gelu':
+        f = a * 0.5 * torch.special.erfc(-a / math.sqrt(2))
+    else:
+        f = 0.5 * a * (1 + torch.tanh(math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)))
+    y = (f * u) @ w_out.t()
+    if b_out is not None:
+        y = y + b_out
+    return y if res is None else y + res
+
+
+FFN_CASES = [  # M, C, F, act, bias, residual
+    (1, 8, 8, 'silu', False, False), (1, 64, 136, 'gelu', True, True), (3, 72, 24, 'gelu_tanh', True, False), (17, 1024, 512, 'silu', True, True),
+    (127, 40, 200, 'gelu', False, True), (256, 256, 256, 'silu', False, False), (257, 264, 680, 'gelu', True, True),
+    (2355, 264, 680, 'gelu_tanh', False, True), (700, 136, 2056, 'silu', True, False), (5000, 64, 48, 'gelu', True, True),
+]
+
+
+def ffn_inputs(M, C, F, bias, residual, dtype):
+    x = rnd(M, C, seed=1, dtype=dtype)
+    w_in, w_out = rnd(2 * F, C, seed=2, dtype=dtype, scale=C ** -0.5), rnd(C, F, seed=3, dtype=dtype, scale=F ** -0.5)
+    b_in, b_out = (rnd(2 * F, seed=4, dtype=dtype, scale=0.3), rnd(C, seed=5, dtype=dtype, scale=0.3)) if bias else (None, None)
+    return [x, w_in, w_out, b_in, b_out, rnd(M, C, seed=6, dtype=dtype) if residual else None]
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('M,C,F,act,bias,residual', FFN_CASES)
+def test_gated_feed_forward_and_gradients(M, C, F, act, bias, residual, dtype):
+    given = ffn_inputs(M, C, F, bias, residual, dtype)
+    leaves = [None if t is None else t.detach().requires_grad_() for t in given]
+    wide = [None if t is None else t.detach().double().requires_grad_() for t in given]
+    y = block.gated_feed_forward(leaves[0], leaves[1], leaves[2], leaves[3], leaves[4], leaves[5], act)
+    plain = block.gated_feed_forward(*given[:5], residual=given[5], activation=act)
+    ref = ffn_ref(*wide, act)
+    assert torch.equal(y, plain) and y.dtype == dtype and y.shape == (M, C)
+    # roundings: the output, h (bf16), then the fp32 sums of C and of F products and ~8 roundings of the activation
+    tol = half_ulp(dtype) * (2 if dtype == BF else 1) + fp32_tol(C) + fp32_tol(F) + 16 * half_ulp(F32)
+    assert rel(y, ref) <= tol, (rel(y, ref), tol)
+    dy = rnd(M, C, seed=9, dtype=dtype)
+    present = [i for i, t in enumerate(leaves) if t is not None]
+    grads = torch.autograd.grad(y, [leaves[i] for i in present], dy)
+    want = torch.autograd.grad(ref, [wide[i] for i in present], dy.double())
+    # bf16: the output, da / du, and the kept a and u they are made from (a's half unit passes through act' and act: their
+    # relative slopes stay below 2 where the values carry weight)
+    for i, g, w in zip(present, grads, want):
+        k = {0: C + 2 * F, 1: C + M, 2: C + M, 3: C + M, 4: M, 5: 0}[i]
+        t = half_ulp(dtype) * (5 if dtype == BF else 1) + 2 * fp32_tol(k + 1) + 32 * half_ulp(F32)
+        assert g.dtype == dtype and g.shape == w.shape and rel(g, w) <= t, (i, rel(g, w), t)
+
+
+def test_gated_feed_forward_columns_one_by_one():
+    """Every operand order of the products with values that name their place: exact in both dtypes, so any element that lands in a
+    wrong row, column or k shows."""
+    for dtype in (BF, F32):
+        for M, C, F in ((300, 136, 264), (72, 520, 96)):
+            x = torch.zeros(M, C, device=DEV, dtype=dtype)
+            rows = torch.arange(M, device=DEV)
+            x[rows, rows % C] = 1
+            w_in = torch.zeros(2 * F, C, device=DEV, dtype=dtype)
+            b_in = torch.zeros(2 * F, device=DEV, dtype=dtype)
+            w_in[:F] = torch.randint(-8, 9, (F, C), device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(dtype)
+            b_in[F:] = 1
+            b_in[:F] = 64          # act(a) = a to fp32 rounding at a >= 56
+            eye = torch.zeros(C, F, device=DEV, dtype=dtype)
+            n = min(C, F)
+            eye[torch.arange(n), torch.arange(n)] = 1
+            y = block.gated_feed_forward(x, w_in, eye, b_in=b_in, activation='gelu')
+            want = torch.zeros(M, C, device=DEV)
+            want[:, :n] = 64 + w_in[:F].t()[rows % C][:, :n].float()
+            assert torch.equal(y.float(), want), (dtype, M, C, F)
+
+
+def test_gated_feed_forward_views_and_empty():
+    x = rnd(3, 5, 128, seed=1, dtype=BF)
+    w_in, w_out = rnd(2 * 64, 72, seed=2, dtype=BF, scale=0.1), rnd(72, 64, seed=3, dtype=BF, scale=0.1)
+    v = x[..., 16:88]
+    want = block.gated_feed_forward(v.contiguous(), w_in, w_out, residual=v.contiguous())
+    assert torch.equal(block.gated_feed_forward(v, w_in, w_out, residual=v), want)
+    assert torch.equal(block.gated_feed_forward(x[..., 3:75], w_in, w_out), block.gated_feed_forward(x[..., 3:75].contiguous(), w_in, w_out))
+    assert torch.equal(block.gated_feed_forward(v.transpose(0, 1), w_in.t().contiguous().t(), w_out, residual=v.transpose(0, 1)), want.transpose(0, 1))
+    one = block.gated_feed_forward(v[1, 2], w_in, w_out)
+    assert one.shape == (72,) and rel(one, ffn_ref(v[1, 2].double()[None], w_in.double(), w_out.double(), None, None, None, 'silu')[0]) <= 2 * half_ulp(BF) + 1e-5
+    e = rnd(0, 72, dtype=BF).requires_grad_()
+    wg = w_in.clone().requires_grad_()
+    y = block.gated_feed_forward(e, wg, w_out)
+    g = torch.autograd.grad(y, (e, wg), torch.empty_like(y))
+    assert y.shape == (0, 72) and g[0].shape == (0, 72) and (g[1] == 0).all()
