@@ -44,6 +44,34 @@ int nd_qk_norm_rope_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                         int D, int R, float eps, int flags, int dtype, nd_stream_t stream);
 int64_t nd_qk_norm_rope_bwd_workspace_floats(int B, int T, int Hq, int Hk, int D);
 
+/* ---- differential attention --------------------------------------------------------------------------------------------- */
+
+#define ND_ATTN_CAUSAL 1 /* query t sees the keys up to t + length - Tq */
+
+/* out = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v with lam = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init
+ * q [B, Tq, H, 2D], k [B, Tk, Hk, 2D] (channels 0 .. D-1: first map, D .. 2D-1: second), v [B, Tk, Hk, Dv], element strides
+ * (batch, token, head), channels contiguous, rows 16-byte aligned.  Query heads h use key head h / (H / Hk).  D, Dv multiples of
+ * 8, at most 128 / 256.  lambda vectors [D] (lambda_sh 0) or [H, D] (lambda_sh D).  key_lengths [B] on the device or NULL: keys
+ * at or past it are neither used nor read as numbers; a query that sees no key gives a zero row.  out [B, Tq, H, Dv] contiguous.
+ * Training: out1, out2 (the two maps' own outputs, like out) and lse [2][B, Tq, H], all or none. */
+int nd_diff_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                      const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const void* lambda_q1, const void* lambda_k1,
+                      const void* lambda_q2, const void* lambda_k2, int64_t lambda_sh, float lambda_init, const int* key_lengths,
+                      void* out, void* out1, void* out2, float* lse, float* workspace, int B, int Tq, int Tk, int H, int Hk, int D, int Dv,
+                      float scale, int flags, int dtype, nd_stream_t stream);
+int64_t nd_diff_attention_workspace_floats(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int dtype); /* may be 0 */
+
+/* gradients of nd_diff_attention from its out1, out2 and lse: dq [B, Tq, H, 2D], dk [B, Tk, Hk, 2D], dv [B, Tk, Hk, Dv]
+ * contiguous; the lambda vectors' (laid out like them) where not NULL.  dout [B, Tq, H, Dv] with its own strides. */
+int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                          const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const void* lambda_q1, const void* lambda_k1,
+                          const void* lambda_q2, const void* lambda_k2, int64_t lambda_sh, float lambda_init, const int* key_lengths,
+                          const void* out1, const void* out2, const float* lse, const void* dout, int64_t do_sb, int64_t do_st,
+                          int64_t do_sh, void* dq, void* dk, void* dv, void* dlambda_q1, void* dlambda_k1, void* dlambda_q2,
+                          void* dlambda_k2, float* workspace, int B, int Tq, int Tk, int H, int Hk, int D, int Dv, float scale, int flags,
+                          int dtype, nd_stream_t stream);
+int64_t nd_diff_attention_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hk);
+
 /* ---- gated feed-forward block ----------------------------------------------------------------------------------------- */
 
 #define ND_ACT_SILU 0

@@ -92,4 +92,24 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[N]) {
     }
 }
 
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// c += a b over one 16-byte piece a lane of either operand: 16 k in bf16 (lane half lh holds k = 8 lh + 0 .. 7), 8 k in fp32
+// (4 lh + 0 .. 3; instruction j takes one k of either half)
+template <typename T>
+__device__ __forceinline__ f32x16 mma_step(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (sizeof(T) == 2) {
+        union { u32x4 u; bf16x8 h; } x, y;
+        x.u = a, y.u = b;
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.h, y.h, c, 0, 0, 0);
+    } else {
+        union { u32x4 u; float f[4]; } x, y;
+        x.u = a, y.u = b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.f[j], y.f[j], c, 0, 0, 0);
+        return c;
+    }
+}
+
 }  // namespace ndb

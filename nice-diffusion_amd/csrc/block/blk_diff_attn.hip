@@ -1,0 +1,457 @@
+// Differential attention, forward:  o = (softmax(s q1 k1^T) - lam softmax(s q2 k2^T)) v,  lam = exp(lq1.lk1) - exp(lq2.lk2) + lam_init
+//
+// q [B, Tq, H, 2D], k [B, Tk, Hk, 2D]: the two halves of a head's channels are the two maps' queries and keys; v [B, Tk, Hk, Dv].
+// The query heads of one key head are rows beside each other: row r of a (batch, key head) is token r / g, head r % g, so one
+// pass over the keys serves all of them.
+//
+// One pass with running maxima and sums for both maps: per 32 keys x 32 rows  S^T = K Q^T  twice, exponentials, O^T += V^T P^T
+// twice (the V fragments are read once).  As in the plain attention kernels a lane holds one row's scores (accumulator as the
+// next product's operand); V^T comes from transposed LDS reads of the row-major tile.  The two outputs stay apart to the end:
+// their scales are only known then.  Alternatively the maps could be joined before the product (two thirds of its operations),
+// at the price of a pass over the scores for the statistics: the same matrix operations and twice the exponentials.
+//   prefill    4 waves x 32 rows, tiles of 64 keys (fp32 with D > 64: 32), two stages, loads straight to LDS
+//   few rows   (g Tq <= 32: single tokens) the waves share the rows and divide the keys of a tile; joined in LDS
+//   wide heads (D > 64) 128 value channels a workgroup, the scores made twice when Dv is above that: both maps' outputs and the
+//              queries of 256 channels do not fit the registers (measured: 290 spilled)
+//   splits     when (batch, key head, row tile) does not fill the chip the keys are divided over workgroups; fp32 partial
+//              outputs, joined in split order by a second launch
+// The maximum a row is scaled by only moves when a score exceeds it by 2^8 (p <= 256: as exact in floating point).  Rounding to
+// bf16 besides the output: the weights p as the second product's operand; their sum is taken from the rounded values.
+#include "blk_diff_attn.h"
+
+namespace ndb {
+
+template <typename T, int HD>
+struct DiffShape {
+    static constexpr int ES = (int)sizeof(T), DV = HD == 128 ? 128 : 2 * HD;      // value channels of a workgroup
+    static constexpr int RBK = 2 * HD * ES, RBV = DV * ES;
+    static constexpr int PH = HD * ES / 16;                  // pieces of one half of a key row
+    static constexpr int NS = PH / 2;                        // steps of a score product
+    static constexpr int NDT = DV / 32;
+    static constexpr int KT_MANY = (ES == 4 && HD == 128) ? 32 : 64;
+    static constexpr int KT_FEW = 128 * (RBK + RBV) <= 65536 ? 128 : (64 * (RBK + RBV) <= 65536 ? 64 : 32);
+};
+
+template <typename T, int HD, bool FEW>
+constexpr int diff_lds_bytes() {
+    using S = DiffShape<T, HD>;
+    constexpr int kt = FEW ? S::KT_FEW : S::KT_MANY, stages = 2 * kt * (S::RBK + S::RBV);
+    constexpr int join = FEW ? 32 * (2 * S::DV + 4) * 4 + (S::KT_FEW / 32) * 32 * 16 : 0;
+    return (stages > join ? stages : join) + DIFF_MAX_GROUP * 4;
+}
+
+template <typename T, int HD, bool FEW>
+constexpr int diff_threads() { return FEW ? 2 * DiffShape<T, HD>::KT_FEW : 256; }
+
+template <typename T, int HD, bool FEW>
+__global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeof(T) >= 256 ? 1 : 2)) diff_attn_kernel(const DiffArgs p) {
+    using S = DiffShape<T, HD>;
+    constexpr int KT = FEW ? S::KT_FEW : S::KT_MANY;
+    constexpr int NW = FEW ? KT / 32 : 4;                    // waves
+    constexpr int STAGE = KT * (S::RBK + S::RBV);
+    using TK = Tile<T, S::RBK>;
+    using TV = Tile<T, S::RBV>;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* const lam_s = reinterpret_cast<float*>(smem + diff_lds_bytes<T, HD, FEW>() - DIFF_MAX_GROUP * 4);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, lh = lane >> 5;
+
+    const int rows = p.Tq * p.g, tiles = (rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
+    const int vblocks = (p.Dv + S::DV - 1) / S::DV;
+    int id = xcd_run(blockIdx.x, gridDim.x);
+    const int per = tiles * p.splits * vblocks, bh = id / per;
+    id -= bh * per;
+    const int vb = HD == 128 ? id / (tiles * p.splits) : 0, dv0 = vb * S::DV, dvn = p.Dv - dv0 < S::DV ? p.Dv - dv0 : S::DV;
+    id -= vb * tiles * p.splits;
+    const int sp = id / tiles, tile = p.causal ? tiles - 1 - (id - sp * tiles) : id - sp * tiles;      // causal: longest rows first
+    const int b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int len = diff_length(p.lengths, b, p.Tk);
+
+    // this lane's row
+    const int r0 = tile * (FEW ? 32 : 128) + (FEW ? 0 : wave * 32);
+    const int r = r0 + l31 < rows ? r0 + l31 : rows - 1;
+    const int t = r / p.g, hg = r - t * p.g, head = hk * p.g + hg;
+    const int seen = p.causal ? t + len - p.Tq + 1 : len;      // keys this row sees (<= 0: none)
+    int last = len;                                            // keys the workgroup needs
+    if (p.causal) {
+        const int rl = (tile + 1) * (FEW ? 32 : 128) - 1 < rows ? (tile + 1) * (FEW ? 32 : 128) - 1 : rows - 1;
+        last = rl / p.g + len - p.Tq + 1;
+    }
+    const int kbeg = sp * p.chunk;
+    int kend = kbeg + p.chunk < last ? kbeg + p.chunk : last;
+
+    for (int h = wave; h < p.g; h += NW) {
+        float e1, e2;
+        diff_lambda<T>(p, hk * p.g + h, lane, e1, e2);
+        if (lane == 0) lam_s[h] = e1 - e2 + p.lam_init;
+    }
+
+    u32x4 q[2][S::NS];
+    {
+        const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q.p) + b * p.q.sb + t * p.q.st + head * p.q.sh);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int c = 0; c < S::NS; ++c) {
+                const int by = (2 * c + lh) * 16;
+                q[m][c] = u32x4{0u, 0u, 0u, 0u};
+                if (by < p.D * S::ES) q[m][c] = *reinterpret_cast<const u32x4*>(qp + m * p.D * S::ES + by);
+            }
+    }
+    f32x16 o[2][S::NDT];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[m][d][e] = 0.f;
+    float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    TileLoad<T, S::RBK, KT, NW> lk;
+    TileLoad<T, S::RBV, KT, NW> lv;
+    lk.template init<S::RBK / 2>(p.k.st * S::ES, p.D * S::ES, wave, lane);
+    lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, wave, lane);
+    const T* kp = static_cast<const T*>(p.k.p) + b * p.k.sb + hk * p.k.sh;
+    const T* vp = static_cast<const T*>(p.v.p) + b * p.v.sb + hk * p.v.sh + dv0;
+    auto fetch = [&](int key, int stage) {                    // keys at or past the sequence's end become zero rows
+        char* at = smem + stage * STAGE;
+        const int64_t n = len - key;
+        lk.load(at, kp + (int64_t)key * p.k.st, ((n - 1) * p.k.st + 2 * p.D) * S::ES, wave);
+        lv.load(at + KT * S::RBK, vp + (int64_t)key * p.v.st, ((n - 1) * p.v.st + dvn) * S::ES, wave);
+    };
+    const int row_base = TK::row_base(lane), col_base = TV::col_base(lane);
+    if (kbeg < kend) fetch(kbeg, 0);
+    int stage = 0;
+    for (int key0 = kbeg; key0 < kend; key0 += KT, stage ^= 1) {
+        // this stage has landed, and every wave is through with the other one
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (key0 + KT < kend) fetch(key0 + KT, stage ^ 1);
+        const char* tk = smem + stage * STAGE;
+        const char* tv = tk + KT * S::RBK;
+#pragma unroll 1
+        for (int sub = FEW ? wave : 0; sub < (FEW ? wave + 1 : KT / 32); ++sub) {
+            const int kb = key0 + sub * 32;
+            if (kb >= kend) break;
+            const int rb = in_loop(row_base), cb = in_loop(col_base), r32 = sub * 32;
+            f32x16 s[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[m][e] = 0.f;
+#pragma unroll
+                for (int c = 0; c < S::NS; ++c) s[m] = mma_step<T>(TK::row(tk + r32 * S::RBK, rb, 0, m * S::PH + 2 * c), q[m][c], s[m]);
+            }
+            // scores past what a row sees: only in the tile that holds a row's end
+            const bool cut = p.causal ? kb + 32 > r0 / p.g + len - p.Tq + 1 : kb + 32 > len;
+            if (cut) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool in = kb + (e & 3) + 8 * (e >> 2) + 4 * lh < seen;
+                    s[0][e] = in ? s[0][e] : -INFINITY;
+                    s[1][e] = in ? s[1][e] : -INFINITY;
+                }
+            }
+            Probs<T> pr[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float top = fmaxf(s[m][0], s[m][1]);
+#pragma unroll
+                for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(s[m][e], s[m][e + 1]), top);
+                top = fmaxf(top, __shfl_xor(top, 32)) * p.c;
+                const bool move = top > mx[m] + 8.f;          // also from -inf
+                if (__builtin_amdgcn_ballot_w64(move) != 0) {
+                    const float a = move ? __builtin_amdgcn_exp2f(mx[m] - top) : 1.f;
+                    mx[m] = move ? top : mx[m];
+                    l[m] *= a;
+#pragma unroll
+                    for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[m][d][e] *= a;
+                }
+                const float ref = mx[m] == -INFINITY ? 0.f : mx[m];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) pr[m].set(e, __builtin_amdgcn_exp2f(fmaf(s[m][e], p.c, -ref)));
+                l[m] += pr[m].sum();                          // this lane half's keys; the halves meet at the end
+            }
+#pragma unroll
+            for (int d = 0; d < S::NDT; ++d) {
+                if constexpr (S::ES == 2) {
+#pragma unroll
+                    for (int s2 = 0; s2 < 2; ++s2) {
+                        union { u32x4 u; bf16x8 h; } a;
+                        a.u = TV::cols(tv + r32 * S::RBV, cb, 16 * s2, d * 32);
+                        o[0][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, pr[0].f[s2], o[0][d], 0, 0, 0);
+                        o[1][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, pr[1].f[s2], o[1][d], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float a = TV::one(tv + r32 * S::RBV, cb, 0, e, d * 32);
+                        o[0][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[0].f[e], o[0][d], 0, 0, 0);
+                        o[1][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[1].f[e], o[1][d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    l[0] += __shfl_xor(l[0], 32);
+    l[1] += __shfl_xor(l[1], 32);
+    __syncthreads();                                          // lam_s is written; the stages are free
+
+    if constexpr (FEW && NW > 1) {
+        // join the waves: a common maximum, then the outputs added in wave order
+        float* ml = reinterpret_cast<float*>(smem);           // [NW][32][4]
+        float* acc = ml + NW * 32 * 4;                        // [32][2 DV + 4]
+        constexpr int LD = 2 * S::DV + 4;
+        if (lh == 0) {
+            ml[(wave * 32 + l31) * 4 + 0] = mx[0];
+            ml[(wave * 32 + l31) * 4 + 1] = l[0];
+            ml[(wave * 32 + l31) * 4 + 2] = mx[1];
+            ml[(wave * 32 + l31) * 4 + 3] = l[1];
+        }
+        __syncthreads();
+        float f[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float top = -INFINITY, sum = 0.f;
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[(w * 32 + l31) * 4 + 2 * m]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            for (int w = 0; w < NW; ++w) sum += ml[(w * 32 + l31) * 4 + 2 * m + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + l31) * 4 + 2 * m] - ref);
+            f[m] = __builtin_amdgcn_exp2f(mx[m] - ref);
+            mx[m] = top;
+            l[m] = sum;
+        }
+        for (int w = 0; w < NW; ++w) {
+            if (wave == w) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            f32x4* a = reinterpret_cast<f32x4*>(acc + l31 * LD + m * S::DV + d * 32 + 8 * g4 + 4 * lh);
+                            f32x4 v = {o[m][d][4 * g4] * f[m], o[m][d][4 * g4 + 1] * f[m], o[m][d][4 * g4 + 2] * f[m], o[m][d][4 * g4 + 3] * f[m]};
+                            if (w) v += *a;
+                            *a = v;
+                            if (w == NW - 1) o[m][d][4 * g4] = v[0], o[m][d][4 * g4 + 1] = v[1], o[m][d][4 * g4 + 2] = v[2], o[m][d][4 * g4 + 3] = v[3];
+                        }
+            }
+            __syncthreads();
+        }
+        if (wave != NW - 1) return;
+    }
+    if (r0 + l31 >= rows) return;
+    if (p.splits > 1) {
+        float* at = p.part + ((int64_t)sp * p.B * p.Hk * rows + (int64_t)bh * rows + r) * (2 * p.Dv + 4);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int dd = d * 32 + 8 * g4 + 4 * lh;
+                    const f32x4 v = {o[m][d][4 * g4], o[m][d][4 * g4 + 1], o[m][d][4 * g4 + 2], o[m][d][4 * g4 + 3]};
+                    if (dd < dvn) *reinterpret_cast<f32x4*>(at + m * p.Dv + dv0 + dd) = v;
+                }
+        if (lh == 0 && vb == 0) *reinterpret_cast<f32x4*>(at + 2 * p.Dv) = f32x4{mx[0], l[0], mx[1], l[1]};
+        return;
+    }
+    const float i1 = l[0] != 0.f ? 1.f / l[0] : 0.f, i2 = l[1] != 0.f ? 1.f / l[1] : 0.f, lam = lam_s[hg];
+    const int64_t orow = ((int64_t)b * p.Tq + t) * p.H + head;
+    if (p.lse && lh == 0 && vb == 0) {
+        p.lse[orow] = l[0] != 0.f ? mx[0] + log2f(l[0]) : INFINITY;
+        p.lse[(int64_t)p.B * p.Tq * p.H + orow] = l[1] != 0.f ? mx[1] + log2f(l[1]) : INFINITY;
+    }
+#pragma unroll
+    for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+            const int dd = d * 32 + 8 * g4 + 4 * lh;
+            if (dd >= dvn) continue;
+            float a[4], c[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = o[0][d][4 * g4 + e] * i1;
+                c[e] = o[1][d][4 * g4 + e] * i2;
+                y[e] = a[e] - lam * c[e];
+            }
+            store_vec<T, 4>(static_cast<T*>(p.out) + orow * p.Dv + dv0 + dd, y);
+            if (p.o1) {
+                store_vec<T, 4>(static_cast<T*>(p.o1) + orow * p.Dv + dv0 + dd, a);
+                store_vec<T, 4>(static_cast<T*>(p.o2) + orow * p.Dv + dv0 + dd, c);
+            }
+        }
+}
+
+// joins the splits of a row: Dv / 4 threads a row
+template <typename T>
+__global__ void __launch_bounds__(256) diff_join_kernel(const DiffArgs p) {
+    const int tpr = p.Dv / 4, rows = p.Tq * p.g;
+    const int64_t all = (int64_t)p.B * p.Hk * rows, row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / tpr;
+    const int dd = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) - row * tpr) * 4;
+    if (row >= all) return;
+    const int bh = (int)(row / rows), r = (int)(row - (int64_t)bh * rows), b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int t = r / p.g, head = hk * p.g + (r - t * p.g);
+    const int LD = 2 * p.Dv + 4;
+    const float* at = p.part + row * LD;
+    const int64_t step = all * LD;
+    float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(at + s * step + 2 * p.Dv);
+        top[0] = fmaxf(top[0], v[0]);
+        top[1] = fmaxf(top[1], v[2]);
+    }
+    f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int s = 0; s < p.splits; ++s) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(at + s * step + 2 * p.Dv);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float f = __builtin_amdgcn_exp2f(v[2 * m] - (top[m] == -INFINITY ? 0.f : top[m]));
+            l[m] += v[2 * m + 1] * f;
+            o[m] += *reinterpret_cast<const f32x4*>(at + s * step + m * p.Dv + dd) * f;
+        }
+    }
+    const T* v[4];
+    float e1 = 0.f, e2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<const T*>(p.lam_vec[i]) + head * p.lam_sh;
+    for (int d = 0; d < p.D; d += 8) {
+        float x[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_vec<T, 8>(v[i] + d, x[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            e1 = fmaf(x[0][e], x[1][e], e1);
+            e2 = fmaf(x[2][e], x[3][e], e2);
+        }
+    }
+    const float lam = expf(e1) - expf(e2) + p.lam_init;
+    const int64_t orow = ((int64_t)b * p.Tq + t) * p.H + head;
+    float a[4], c[4], y[4];
+    const float i1 = l[0] != 0.f ? 1.f / l[0] : 0.f, i2 = l[1] != 0.f ? 1.f / l[1] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        a[e] = o[0][e] * i1;
+        c[e] = o[1][e] * i2;
+        y[e] = a[e] - lam * c[e];
+    }
+    store_vec<T, 4>(static_cast<T*>(p.out) + orow * p.Dv + dd, y);
+    if (p.o1) {
+        store_vec<T, 4>(static_cast<T*>(p.o1) + orow * p.Dv + dd, a);
+        store_vec<T, 4>(static_cast<T*>(p.o2) + orow * p.Dv + dd, c);
+    }
+    if (p.lse && dd == 0) {
+        p.lse[orow] = l[0] != 0.f ? top[0] + log2f(l[0]) : INFINITY;
+        p.lse[(int64_t)p.B * p.Tq * p.H + orow] = l[1] != 0.f ? top[1] + log2f(l[1]) : INFINITY;
+    }
+}
+
+// padded head dim of the kernels: the smallest of 32 / 64 / 128 that holds D and half of Dv
+int diff_head_dim(int D, int Dv) {
+    const int n = D > (Dv + 1) / 2 ? D : (Dv + 1) / 2;
+    return n <= 32 ? 32 : (n <= 64 ? 64 : 128);
+}
+
+struct DiffPlan {
+    bool few;
+    int splits, chunk;
+};
+
+// One workgroup per (batch, key head, row tile) unless that leaves CUs idle: then the keys are divided until ~512 workgroups
+// exist (few rows: ~256, one to a CU by their LDS), no split under 256 keys
+static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv) {
+    const int g = H / Hk, rows = Tq * g, hd = diff_head_dim(D, Dv);
+    DiffPlan pl{rows <= 32, 1, Tk};
+    const int kt = 128;                                       // whole tiles of every variant
+    const int64_t units = (int64_t)B * Hk * (pl.few ? 1 : (rows + 127) / 128) * (hd == 128 ? (Dv + 127) / 128 : 1);
+    const int64_t want = (pl.few ? 256 : 512) / (units < 1 ? 1 : units);
+    int64_t splits = want < 1 ? 1 : want;
+    const int64_t most = (Tk + 255) / 256;
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;
+    const int64_t chunk = ((Tk + splits - 1) / splits + kt - 1) / kt * kt;
+    pl.chunk = (int)chunk;
+    pl.splits = (int)((Tk + chunk - 1) / chunk);
+    if (pl.splits < 1) pl.splits = 1;
+    return pl;
+}
+
+template <typename T, int HD, bool FEW>
+static int launch_diff(const char* fn, const DiffArgs& a, hipStream_t st) {
+    auto kern = diff_attn_kernel<T, HD, FEW>;
+    static bool attr_set[kMaxDevices] = {};
+    if (int rc = ensure_max_lds(reinterpret_cast<const void*>(kern), attr_set, fn)) return rc;
+    const int rows = a.Tq * a.g, per = FEW ? 32 : 128;
+    const int vblocks = (a.Dv + DiffShape<T, HD>::DV - 1) / DiffShape<T, HD>::DV;
+    const int64_t blocks = (int64_t)a.B * a.Hk * ((rows + per - 1) / per) * a.splits * vblocks;
+    NDB_REQUIRE(blocks <= (1 << 24), fn, "too many workgroups for one launch");
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(diff_threads<T, HD, FEW>()), (diff_lds_bytes<T, HD, FEW>()), st, a);
+    if (a.splits > 1) {
+        const int64_t threads = (int64_t)a.B * a.Hk * rows * (a.Dv / 4);
+        hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+    }
+    return check_launch(fn);
+}
+
+template <typename T>
+static int dispatch_diff(const char* fn, const DiffArgs& a, bool few, hipStream_t st) {
+    switch (diff_head_dim(a.D, a.Dv)) {
+        case 32: return few ? launch_diff<T, 32, true>(fn, a, st) : launch_diff<T, 32, false>(fn, a, st);
+        case 64: return few ? launch_diff<T, 64, true>(fn, a, st) : launch_diff<T, 64, false>(fn, a, st);
+        default: return few ? launch_diff<T, 128, true>(fn, a, st) : launch_diff<T, 128, false>(fn, a, st);
+    }
+}
+
+int diff_check(const char* fn, const DiffArgs& a, int dtype) {
+    NDB_REQUIRE(dtype == ND_DT_F32 || dtype == ND_DT_BF16, fn, "dtype must be ND_DT_F32 or ND_DT_BF16");
+    NDB_REQUIRE(a.B > 0 && a.Tq > 0 && a.Tk > 0 && a.H > 0 && a.Hk > 0, fn, "sizes must be positive");
+    NDB_REQUIRE(a.H % a.Hk == 0 && a.H / a.Hk <= DIFF_MAX_GROUP, fn, "query heads must be a multiple of the key heads, at most 64 times as many");
+    NDB_REQUIRE(a.D > 0 && a.D % 8 == 0 && a.D <= 128, fn, "head dim must be a multiple of 8 and at most 128");
+    NDB_REQUIRE(a.Dv > 0 && a.Dv % 8 == 0 && a.Dv <= 256, fn, "value dim must be a multiple of 8 and at most 256");
+    NDB_REQUIRE((int64_t)a.Tq * a.H < (1LL << 30) && a.Tk < (1 << 30), fn, "too many tokens");
+    NDB_REQUIRE(a.scale > 0.f, fn, "scale must be positive");
+    const int per = dtype == ND_DT_BF16 ? 8 : 4;
+    const DiffTensor* t[3] = {&a.q, &a.k, &a.v};
+    for (const DiffTensor* x : t) {
+        NDB_REQUIRE(x->p, fn, "null pointer");
+        NDB_REQUIRE(aligned_to(x->p, 16) && x->sb % per == 0 && x->st % per == 0 && x->sh % per == 0, fn, "rows must be 16-byte aligned");
+        NDB_REQUIRE(x->st >= 0 && x->st <= (1 << 22), fn, "token stride must be 0 .. 2^22 elements");
+    }
+    for (const void* v : a.lam_vec) NDB_REQUIRE(v && aligned_to(v, 16), fn, "lambda vectors must be given, 16-byte aligned");
+    return ND_OK;
+}
+
+}  // namespace ndb
+
+using namespace ndb;
+
+extern "C" int64_t nd_diff_attention_workspace_floats(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int dtype) {
+    if (B <= 0 || Tq <= 0 || Tk <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || D > 128 || Dv <= 0 || Dv > 256) return -1;
+    const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv);
+    return pl.splits > 1 ? (int64_t)pl.splits * B * Tq * H * (2 * Dv + 4) : 0;
+}
+
+extern "C" int nd_diff_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
+                                 int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const void* lambda_q1,
+                                 const void* lambda_k1, const void* lambda_q2, const void* lambda_k2, int64_t lambda_sh, float lambda_init,
+                                 const int* key_lengths, void* out, void* out1, void* out2, float* lse, float* workspace, int B, int Tq,
+                                 int Tk, int H, int Hk, int D, int Dv, float scale, int flags, int dtype, nd_stream_t stream) {
+    const char* fn = "nd_diff_attention";
+    DiffArgs a{};
+    a.q = {q, q_sb, q_st, q_sh}, a.k = {k, k_sb, k_st, k_sh}, a.v = {v, v_sb, v_st, v_sh};
+    a.lam_vec[0] = lambda_q1, a.lam_vec[1] = lambda_k1, a.lam_vec[2] = lambda_q2, a.lam_vec[3] = lambda_k2;
+    a.lam_sh = lambda_sh, a.lam_init = lambda_init, a.lengths = key_lengths;
+    a.out = out, a.o1 = out1, a.o2 = out2, a.lse = lse, a.part = workspace;
+    a.B = B, a.Tq = Tq, a.Tk = Tk, a.H = H, a.Hk = Hk, a.D = D, a.Dv = Dv, a.causal = flags & ND_ATTN_CAUSAL;
+    a.scale = scale, a.c = scale * 1.4426950408889634f;
+    if (int rc = diff_check(fn, a, dtype)) return rc;
+    a.g = H / Hk;
+    NDB_REQUIRE(out && aligned_to(out, 16) && (!out1 || (out2 && lse && aligned_to(out1, 16) && aligned_to(out2, 16))), fn, "outputs missing or not 16-byte aligned");
+    const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv);
+    a.splits = pl.splits, a.chunk = pl.chunk;
+    NDB_REQUIRE(pl.splits == 1 || (workspace && aligned_to(workspace, 16)), fn, "workspace missing");
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return dtype == ND_DT_BF16 ? dispatch_diff<__bf16>(fn, a, pl.few, st) : dispatch_diff<float>(fn, a, pl.few, st);
+}

@@ -54,9 +54,6 @@ __device__ __forceinline__ void gemm_tile(int lin, int total, int tiles_m, int t
     tm = first + id - tn * rows;
 }
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
 // one operand of a workgroup tile: its share of the loads, and its fragments
 template <typename T, int TI, bool KMAJOR>
 struct GemmOperand {
@@ -157,21 +154,6 @@ struct GemmOperand {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ f32x16 gemm_mma(u32x4 a, u32x4 b, f32x16 c) {
-    if constexpr (sizeof(T) == 2) {
-        union { u32x4 u; bf16x8 h; } x, y;
-        x.u = a, y.u = b;
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.h, y.h, c, 0, 0, 0);
-    } else {
-        union { u32x4 u; float f[4]; } x, y;
-        x.u = a, y.u = b;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.f[j], y.f[j], c, 0, 0, 0);
-        return c;
-    }
-}
-
 template <int TI>
 constexpr int gemm_lds_bytes() { return 2 * 2 * 64 * TI * 128; }
 
@@ -255,7 +237,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, TI == 4 ? 1 : 2) gemm_kernel(con
 #pragma unroll
             for (int a = 0; a < TI; ++a)
 #pragma unroll
-                for (int b = 0; b < TI; ++b) acc[a][b] = gemm_mma<T>(fw[c][a], fx[c][b], acc[a][b]);
+                for (int b = 0; b < TI; ++b) acc[a][b] = mma_step<T>(fw[c][a], fx[c][b], acc[a][b]);
         }
     }
     // a lane's piece: row m, columns n .. n + 3

@@ -29,6 +29,7 @@ STEP_PER_IMAGE = 2
 
 # flags of libnd_block.so (mirror include/nd_block.h)
 ROPE_INTERLEAVED = 1
+ATTN_CAUSAL = 1
 ACT_SILU = 0
 ACT_GELU = 1
 ACT_GELU_TANH = 2
@@ -151,6 +152,10 @@ BLOCK_SIGNATURES = {
     'nd_qk_norm_rope': (_T3 * 2 + [_vp, _vp, _vp, _vp, _i64] + _T3 * 2 + [_i] * 6 + [_f, _i, _i, _vp], _i),
     'nd_qk_norm_rope_bwd': (_T3 * 2 + [_vp, _vp, _vp, _vp, _i64] + _T3 * 4 + [_vp, _vp, _vp] + [_i] * 6 + [_f, _i, _i, _vp], _i),
     'nd_qk_norm_rope_bwd_workspace_floats': ([_i] * 5, _i64),
+    'nd_diff_attention': (_T3 * 3 + [_vp] * 4 + [_i64, _f] + [_vp] * 6 + [_i] * 7 + [_f, _i, _i, _vp], _i),
+    'nd_diff_attention_workspace_floats': ([_i] * 8, _i64),
+    'nd_diff_attention_bwd': (_T3 * 3 + [_vp] * 4 + [_i64, _f] + [_vp] * 4 + _T3 + [_vp] * 8 + [_i] * 7 + [_f, _i, _i, _vp], _i),
+    'nd_diff_attention_bwd_workspace_floats': ([_i] * 5, _i64),
     'nd_gated_ffn': ([_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp] + [_i] * 5 + [_vp], _i),
     'nd_gated_ffn_workspace_floats': ([_i] * 4, _i64),
     'nd_gated_ffn_bwd': ([_vp, _i64, _vp, _i64] + [_vp] * 11 + [_i] * 5 + [_vp], _i),

@@ -65,6 +65,18 @@ def _call(name, device, *args):
     _hip.check_block(rc, name)
 
 
+def _aligned(t):
+    """A contiguous parameter on a 16-byte boundary."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _floats(n, device):
+    return torch.empty(n, dtype=torch.float32, device=device) if n > 0 else None
+
+
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -212,6 +224,111 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
     return qo, ko
 
 
+# -------------------------------------------------------------------------------------------- differential attention
+def _attn_rows(t):
+    """``t`` [B, T, heads, channels] as the kernels read it: contiguous channels, every row on a 16-byte boundary (else a copy)."""
+    per = 16 // t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % per for s in _strides(t)) or not 0 <= _strides(t)[1] <= 1 << 22:
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _diff_args(q, k, v, lams, lambda_init, lengths):
+    per_head = lams[0].dim() == 2
+    return [q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), *(t.data_ptr() for t in lams),
+            lams[0].shape[-1] if per_head else 0, lambda_init, _hip.ptr(lengths)]
+
+
+def _diff_sizes(q, k, v):
+    return [q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3] // 2, v.shape[3]]
+
+
+def _launch_diff(q, k, v, lams, lambda_init, scale, lengths, causal, keep):
+    B, Tq, Tk, H, Hk, D, Dv = sizes = _diff_sizes(q, k, v)
+    new = dict(dtype=q.dtype, device=q.device)
+    out = torch.empty(B, Tq, H, Dv, **new)
+    o1, o2, lse = (torch.empty(B, Tq, H, Dv, **new), torch.empty(B, Tq, H, Dv, **new), _floats(2 * B * Tq * H, q.device)) if keep else (None,) * 3
+    ws = _floats(_hip.load_block().nd_diff_attention_workspace_floats(*sizes, _DT[q.dtype]), q.device)
+    _call('nd_diff_attention', q.device, *_diff_args(q, k, v, lams, lambda_init, lengths), out.data_ptr(), _hip.ptr(o1), _hip.ptr(o2),
+          _hip.ptr(lse), _hip.ptr(ws), *sizes, scale, _hip.ATTN_CAUSAL if causal else 0, _DT[q.dtype])
+    return out, o1, o2, lse
+
+
+class _DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lq1, lk1, lq2, lk2, lambda_init, scale, lengths, causal):
+        q, k, v = _attn_rows(q), _attn_rows(k), _attn_rows(v)
+        lams = [_aligned(t) for t in (lq1, lk1, lq2, lk2)]
+        out, o1, o2, lse = _launch_diff(q, k, v, lams, lambda_init, scale, lengths, causal, True)
+        ctx.save_for_backward(q, k, v, *lams, lengths, o1, o2, lse)
+        ctx.lambda_init, ctx.scale, ctx.causal = lambda_init, scale, causal
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, lq1, lk1, lq2, lk2, lengths, o1, o2, lse = ctx.saved_tensors
+        lams = [lq1, lk1, lq2, lk2]
+        sizes = _diff_sizes(q, k, v)
+        dout = _attn_rows(dout)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dl = [torch.empty_like(t) if n else None for t, n in zip(lams, ctx.needs_input_grad[3:7])]
+        ws = _floats(_hip.load_block().nd_diff_attention_bwd_workspace_floats(*sizes[:5]), q.device)
+        _call('nd_diff_attention_bwd', q.device, *_diff_args(q, k, v, lams, ctx.lambda_init, lengths), o1.data_ptr(), o2.data_ptr(),
+              lse.data_ptr(), dout.data_ptr(), *_strides(dout), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *(_hip.ptr(t) for t in dl),
+              ws.data_ptr(), *sizes, ctx.scale, _hip.ATTN_CAUSAL if ctx.causal else 0, _DT[q.dtype])
+        return (dq, dk, dv, *dl, None, None, None, None)
+
+
+def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, lambda_init=0.8, scale=None, key_lengths=None, causal=False):
+    """``(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v`` with ``lam = exp(lq1.lk1) - exp(lq2.lk2) + lambda_init``.
+
+    q [B, Tq, H, 2 D], k [B, Tk, Hk, 2 D]: the first D channels of a head are the first map's, the rest the second's; v
+    [B, Tk, Hk, Dv].  Query head h reads key head h // (H / Hk).  D and Dv multiples of 8, at most 128 and 256.  Any strides (views
+    of a packed qkv row); a cache that is longer than its contents is passed whole with ``key_lengths``.  The lambda vectors are [D]
+    (one layer's) or [H, D] (each head its own).  scale defaults to D ** -0.5 and must be positive.
+
+    key_lengths [B] (int32 or int64, on the GPU): keys at or past it take no part, whatever their memory holds; values are held
+    to 0 .. Tk.  causal: query t sees the keys up to t + length - Tq (the queries are the sequence's last).  A query that sees no
+    key gives a zero row and no gradient.  Returns [B, Tq, H, Dv], contiguous.  Few query rows (Tq H / Hk <= 32, single tokens) have
+    a form of their own that divides the keys."""
+    if q.dim() != 4 or q.shape[3] % 2:
+        raise ValueError('q has shape {}, expected [B, Tq, H, 2 D]'.format(tuple(q.shape)))
+    B, Tq, H, D = q.shape[0], q.shape[1], q.shape[2], q.shape[3] // 2
+    _shape(k, 'k', B, None, None, 2 * D)
+    Tk, Hk = k.shape[1], k.shape[2]
+    _shape(v, 'v', B, Tk, Hk, None)
+    Dv = v.shape[3]
+    lams = (lambda_q1, lambda_k1, lambda_q2, lambda_k2)
+    names = ('lambda_q1', 'lambda_k1', 'lambda_q2', 'lambda_k2')
+    if tuple(lambda_q1.shape) not in ((D,), (H, D)):
+        raise ValueError('lambda_q1 has shape {}, expected [{}] or [{}, {}]'.format(tuple(lambda_q1.shape), D, H, D))
+    for n, t in zip(names, lams):
+        _shape(t, n, *lambda_q1.shape)
+    _check(('q', q), k=k, v=v, **dict(zip(names, lams)))
+    if D == 0 or D % 8 or D > 128 or Dv == 0 or Dv % 8 or Dv > 256:
+        raise ValueError('D ({}) and Dv ({}) must be positive multiples of 8, at most 128 and 256'.format(D, Dv))
+    if H == 0 or Hk == 0 or H % Hk or H // Hk > 64:
+        raise ValueError('{} query heads do not divide among {} key heads (at most 64 each)'.format(H, Hk))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < float('inf'):
+        raise ValueError('scale must be positive, got {}'.format(scale))
+    if key_lengths is not None:
+        _shape(key_lengths, 'key_lengths', B)
+        if key_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError('key_lengths is {}: int32 or int64 expected'.format(key_lengths.dtype))
+        if key_lengths.device != q.device:
+            raise ValueError('key_lengths lives on {}, q on {}'.format(key_lengths.device, q.device))
+        key_lengths = (key_lengths.clamp(0, Tk) if key_lengths.dtype == torch.int64 else key_lengths).to(torch.int32).contiguous()
+    if B == 0 or Tq == 0 or Tk == 0:        # nothing to see: zeros that every input's gradient (zero) flows through
+        out = torch.zeros(B, Tq, H, Dv, dtype=q.dtype, device=q.device)
+        return out + 0 * sum(t.sum() for t in (q, k, v) + lams) if _wants_grad(q, k, v, *lams) else out
+    if _wants_grad(q, k, v, *lams):
+        return _DiffAttention.apply(q, k, v, *lams, float(lambda_init), scale, key_lengths, bool(causal))
+    return _launch_diff(_attn_rows(q), _attn_rows(k), _attn_rows(v), [_aligned(t) for t in lams], float(lambda_init), scale, key_lengths,
+                        bool(causal), False)[0]
+
+
 # ------------------------------------------------------------------------------------------------ gated feed-forward
 _ACTS = {'silu': _hip.ACT_SILU, 'gelu': _hip.ACT_GELU, 'gelu_tanh': _hip.ACT_GELU_TANH}
 
@@ -226,18 +343,6 @@ def _matrix(t, cols):
 
 def _ld(m):
     return m.shape[1] if m.shape[0] == 1 else m.stride(0)
-
-
-def _aligned(t):
-    """A contiguous parameter on a 16-byte boundary."""
-    if t is None:
-        return None
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _floats(n, device):
-    return torch.empty(n, dtype=torch.float32, device=device) if n > 0 else None
 
 
 def _launch_ffn(x, w_in, b_in, w_out, b_out, res, act, keep):

@@ -262,3 +262,172 @@ def test_gated_feed_forward_views_and_empty():
     y = block.gated_feed_forward(e, wg, w_out)
     g = torch.autograd.grad(y, (e, wg), torch.empty_like(y))
     assert y.shape == (0, 72) and g[0].shape == (0, 72) and (g[1] == 0).all()
+
+
+# -------------------------------------------------------------------------------------------- differential_attention
+def diff_ref(q, k, v, lams, lam_init, scale, lengths, causal, u, dout=None):
+    """Outputs and gradients in float64 with, for each, the 2-norm that its error may have when the weights, dS and the kept maps'
+    outputs are rounded by at most u relative and a score's exponential by eps (fp32)."""
+    B, Tq, H, _ = q.shape
+    Tk, Hk, D, Dv = k.shape[1], k.shape[2], q.shape[3] // 2, v.shape[3]
+    per_head = lams[0].dim() == 2
+    out = torch.zeros(B, Tq, H, Dv, dtype=torch.float64, device=q.device)
+    e_out = torch.zeros_like(out)
+    dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    e_q, e_k, e_v = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    dl, e_l = [torch.zeros_like(t) for t in lams], [torch.zeros_like(t) for t in lams]
+    for b in range(B):
+        n = lengths[b]
+        for h in range(H):
+            a1, b1, a2, b2 = (t[h] if per_head else t for t in lams)
+            x1, x2 = (a1 * b1).sum().exp(), (a2 * b2).sum().exp()
+            lam = x1 - x2 + lam_init
+            if n == 0:
+                continue
+            g = h // (H // Hk)
+            kk, vv = k[b, :n, g], v[b, :n, g]
+            ps = []
+            for m in range(2):
+                s = q[b, :, h, m * D:(m + 1) * D] @ kk[:, m * D:(m + 1) * D].t() * scale
+                if causal:
+                    s = s.masked_fill(torch.ones(Tq, n, dtype=torch.bool, device=q.device).triu(n - Tq + 1), -math.inf)
+                ps.append(torch.softmax(s, -1).nan_to_num(0.0))
+                smax = s[s > -math.inf].abs().max().item() if (s > -math.inf).any() else 0.0
+            eps = (smax + 8) * 4 * half_ulp(F32) * math.sqrt(D)
+            p1, p2 = ps
+            o1, o2 = p1 @ vv, p2 @ vv
+            out[b, :, h] = o1 - lam * o2
+            e_out[b, :, h] = (u + eps) * ((p1 + abs(lam) * p2) @ vv.abs())
+            if dout is None:
+                continue
+            do = dout[b, :, h]
+            dp = do @ vv.t()
+            pd = p1 - lam * p2
+            dv[b, :n, g] += pd.t() @ do
+            e_v[b, :n, g] += (u * pd.abs() + eps * (p1 + abs(lam) * p2)).t() @ do.abs()
+            dlam = -(p2 * dp).sum()
+            e_lam = (p2 * eps * dp.abs()).sum() + 4 * math.sqrt(Dv) * half_ulp(F32) * (p2 * (do.abs() @ vv.abs().t())).sum()
+            for i, (val, o) in enumerate(((x1, b1), (x1, a1), (-x2, b2), (-x2, a2))):
+                tgt, etgt = (dl[i][h], e_l[i][h]) if per_head else (dl[i], e_l[i])
+                tgt += dlam * val * o
+                etgt += e_lam * val.abs() * o.abs()
+            for m, (p, o, f) in enumerate(((p1, o1, 1.0), (p2, o2, -lam))):
+                c = (do * o).sum(-1, keepdim=True)
+                e_c = (u + eps) * (do.abs() * o.abs()).sum(-1, keepdim=True)
+                ds = f * p * (dp - c) * scale
+                e_ds = u * ds.abs() + abs(f) * p * scale * (e_c + eps * (dp.abs() + c.abs()))
+                half = slice(m * D, (m + 1) * D)
+                if n > 1:
+                    dq[b, :, h, half] = ds @ kk[:, half]
+                    e_q[b, :, h, half] = e_ds @ kk[:, half].abs()
+                    dk[b, :n, g, half] += ds.t() @ q[b, :, h, half]
+                    e_k[b, :n, g, half] += e_ds.t() @ q[b, :, h, half].abs()
+    return (out, e_out), [(dq, e_q), (dk, e_k), (dv, e_v)] + list(zip(dl, e_l))
+
+
+DIFF_CASES = [  # B, Tq, Tk, H, Hk, D, Dv, lengths, causal, per head
+    (1, 1, 1, 1, 1, 8, 8, None, False, False), (2, 64, 64, 2, 2, 32, 64, None, False, False), (2, 64, 64, 2, 2, 32, 64, None, True, False),
+    (3, 49, 49, 4, 2, 32, 64, (49, 17, 0), False, True), (2, 130, 130, 2, 1, 64, 128, (130, 65), True, True), (1, 257, 300, 2, 2, 64, 128, None, True, False),
+    (2, 1, 700, 8, 2, 64, 128, (700, 1), False, False), (3, 3, 1500, 4, 4, 32, 64, (1500, 2, 0), True, False), (1, 1, 5000, 16, 1, 128, 256, None, False, True),
+    (2, 70, 33, 3, 3, 128, 256, None, True, False), (1, 100, 90, 2, 1, 96, 192, (64,), False, False), (2, 33, 65, 2, 2, 24, 40, (65, 31), False, True),
+    (1, 40, 40, 6, 2, 128, 128, None, True, False), (1, 600, 600, 1, 1, 40, 80, None, False, False), (2, 5, 2, 2, 2, 16, 16, (1, 2), False, False),
+    (1, 4, 97, 32, 4, 56, 112, None, True, False),
+]
+
+
+def diff_inputs(B, Tq, Tk, H, Hk, D, Dv, lengths, per_head, dtype):
+    q, k, v = rnd(B, Tq, H, 2 * D, seed=1, dtype=dtype), rnd(B, Tk, Hk, 2 * D, seed=2, dtype=dtype), rnd(B, Tk, Hk, Dv, seed=3, dtype=dtype)
+    k[0, Tk // 2] *= 3          # a spiky key: the running maximum moves
+    lams = [rnd(*((H, D) if per_head else (D,)), seed=4 + i, dtype=dtype, scale=0.2) for i in range(4)]
+    return q, k, v, lams, None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+
+
+def within(got, ref, err, dtype, slack=1.0):
+    """2-norm of the difference against the derived bound plus the output's own rounding."""
+    return (got.double() - ref).norm().item() <= slack * (err.norm().item() + half_ulp(dtype) * ref.norm().item()) * (1 + 1e-6) + 1e-30
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('B,Tq,Tk,H,Hk,D,Dv,lengths,causal,per_head', DIFF_CASES)
+def test_differential_attention_and_gradients(B, Tq, Tk, H, Hk, D, Dv, lengths, causal, per_head, dtype):
+    q, k, v, lams, ln = diff_inputs(B, Tq, Tk, H, Hk, D, Dv, lengths, per_head, dtype)
+    if lengths is not None:          # what lies behind a sequence's end is not looked at
+        for b, n in enumerate(lengths):
+            k[b, n:] = math.nan
+            v[b, n:] = math.inf
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, *lams)]
+    out = block.differential_attention(*leaves, lambda_init=0.6, key_lengths=ln, causal=causal)
+    plain = block.differential_attention(q, k, v, *lams, lambda_init=0.6, key_lengths=ln, causal=causal)
+    assert torch.equal(out, plain) and out.dtype == dtype and out.shape == (B, Tq, H, Dv)
+    dout = rnd(B, Tq, H, Dv, seed=11, dtype=dtype)
+    u = half_ulp(BF) if dtype == BF else 0.0
+    full = lengths or (Tk,) * B
+    (ref, err), grads = diff_ref(*(t.double() for t in (q, k, v)), [t.double() for t in lams], 0.6, D ** -0.5, full, causal, u, dout.double())
+    assert within(out, ref, err, dtype), ((out.double() - ref).norm() / ref.norm(), err.norm() / ref.norm())
+    for b in range(B):                # rows that see nothing
+        blind = Tq if full[b] == 0 else (max(0, Tq - full[b]) if causal else 0)
+        assert (out[b, :blind] == 0).all()
+    got = torch.autograd.grad(out, leaves, dout)
+    for i, (g, (r, e)) in enumerate(zip(got, grads)):
+        assert g.dtype == dtype and within(g, r, e, dtype), (i, (g.double() - r).norm() / r.norm(), e.norm() / r.norm())
+    for b in range(B):
+        assert (got[1][b, full[b]:] == 0).all() and (got[2][b, full[b]:] == 0).all()
+        if full[b] <= 1:
+            assert (got[0][b] == 0).all() and (got[1][b] == 0).all()
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_differential_attention_in_a_packed_row(dtype):
+    B, T, H, D = 2, 77, 3, 32
+    row = rnd(B, T, H, 3, 2 * D, seed=1, dtype=dtype)          # q, k, v of each head beside each other
+    q, k, v = row.unbind(3)
+    lams = [rnd(D, seed=4 + i, dtype=dtype, scale=0.2) for i in range(4)]
+    a = block.differential_attention(q, k, v, *lams)
+    b = block.differential_attention(q.contiguous(), k.contiguous(), v.contiguous(), *lams)
+    assert torch.equal(a, b)
+    # rows off the 16-byte grid and transposed channels are copied
+    wide = rnd(B, T, H, 2 * D + 1, seed=5, dtype=dtype)
+    assert torch.equal(block.differential_attention(wide[..., 1:], k, v, *lams), block.differential_attention(wide[..., 1:].contiguous(), k, v, *lams))
+    # shared keys (a batch of one, expanded) and int64 lengths
+    ks, vs = k[:1].expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1)
+    ln = torch.tensor([77, 20], device=DEV)
+    c = block.differential_attention(q, ks, vs, *lams, key_lengths=ln)
+    assert torch.equal(c, block.differential_attention(q, ks.contiguous(), vs.contiguous(), *lams, key_lengths=ln.int()))
+    leaf = k[:1].clone().requires_grad_()
+    g, = torch.autograd.grad(block.differential_attention(q, leaf.expand(B, -1, -1, -1), vs, *lams, key_lengths=ln), leaf, a)
+    assert g.shape == leaf.shape and torch.isfinite(g).all()
+
+
+def test_differential_attention_splits_agree_with_one_pass():
+    """The same queries alone (keys divided among waves and workgroups) and among many (one pass)."""
+    for dtype in (BF, F32):
+        q, k, v, lams, _ = diff_inputs(1, 512, 2048, 4, 2, 64, 128, None, False, dtype)
+        many = block.differential_attention(q, k, v, *lams)
+        one = block.differential_attention(q[:, 100:101], k, v, *lams)
+        assert rel(one, many[:, 100:101].double()) <= (2.5 if dtype == BF else 16) * half_ulp(dtype)
+
+
+def test_differential_attention_gradient_against_differences():
+    q, k, v, lams, _ = diff_inputs(1, 5, 6, 2, 1, 8, 16, None, False, F32)
+    leaves = [t.requires_grad_() for t in (q, k, v, *lams)]
+    dout = rnd(1, 5, 2, 16, seed=8)
+    grads = torch.autograd.grad(block.differential_attention(*leaves, causal=True), leaves, dout)
+    step = 2.0 ** -7
+    for i, t in enumerate(leaves):
+        d = rnd(*t.shape, seed=20 + i, scale=0.3)
+        with torch.no_grad():
+            f = [(block.differential_attention(*[x + sgn * step * d if j == i else x for j, x in enumerate(leaves)], causal=True).double() * dout.double()).sum()
+                 for sgn in (1, -1)]
+        num, ana = ((f[0] - f[1]) / (2 * step)).item(), (grads[i].double() * d.double()).sum().item()
+        # central difference: third derivatives of O(100) / 6 times step^2, rounding 100 * 2^-24 / step
+        assert abs(num - ana) <= 100 / 6 * step ** 2 + 100 * 2.0 ** -24 / step + 1e-3 * abs(ana), (i, num, ana)
+
+
+def test_differential_attention_empty():
+    lams = [rnd(8, seed=i).requires_grad_() for i in range(4)]
+    for B, Tq, Tk in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        q, k, v = (torch.randn(B, t, 2, 16, device=DEV, requires_grad=True) for t in (Tq, Tk, Tk))
+        o = block.differential_attention(q, k, v, *lams)
+        assert o.shape == (B, Tq, 2, 16) and (o == 0).all()
+        for g, t in zip(torch.autograd.grad(o.sum(), (q, k, v, *lams)), (q, k, v, *lams)):
+            assert g.shape == t.shape and (g == 0).all()
