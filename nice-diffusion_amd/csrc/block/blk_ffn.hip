@@ -14,16 +14,28 @@
 
 namespace ndb {
 
-template <int ACT>
+// f = act(a), df = act'(a).  The normal distribution of gelu: fp32 calls take the library's error function; in bf16 calls, whose
+// results carry 8 bits, Hastings' rational form serves both it and the slope with one exponential (Abramowitz and Stegun 7.1.26:
+// erfc(x) = t P(t) exp(-x^2), t = 1 / (1 + 0.3275911 x), to 1.5e-7): with erff the epilogue took 60 of the 265 us of the first
+// product of ffn at 65536 x 384 x 1024.
+template <typename T, int ACT>
 __device__ __forceinline__ void act_and_slope(float a, float& f, float& df) {
     if constexpr (ACT == ND_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.f + __expf(-a));
         f = a * s;
         df = s * (1.f + a * (1.f - s));
     } else if constexpr (ACT == ND_ACT_GELU) {
-        const float cdf = 0.5f * (1.f + erff(a * 0.70710678118654752f));
+        float cdf, pdf = __expf(-0.5f * a * a);
+        if constexpr (sizeof(T) == 2) {
+            const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(a), 1.f));
+            const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+            const float tail = 0.5f * poly * pdf;             // of the normal distribution beyond |a|
+            cdf = a < 0.f ? tail : 1.f - tail;
+        } else {
+            cdf = 0.5f * (1.f + erff(a * 0.70710678118654752f));
+        }
         f = a * cdf;
-        df = cdf + a * 0.3989422804014327f * __expf(-0.5f * a * a);
+        df = fmaf(a * 0.3989422804014327f, pdf, cdf);
     } else {      // 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z)),  z = sqrt(2 / pi) (a + 0.044715 a^3)
         const float z2 = 1.5957691216057308f * a * (1.f + 0.044715f * a * a);
         const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z2));
@@ -32,42 +44,66 @@ __device__ __forceinline__ void act_and_slope(float a, float& f, float& df) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p) {
-    float t[4];
-    load_vec<T, 4>(p, t);
-    return f32x4{t[0], t[1], t[2], t[3]};
-}
+// Epilogues: columns(n) what a lane needs for its 8 columns, row(m, n) what it reads for one row of them (requested ahead of the
+// row's turn), store(...) the rest.
+struct None {};
 
 template <typename T>
-__device__ __forceinline__ void store4(T* p, const f32x4& v) {
-    const float t[4] = {v[0], v[1], v[2], v[3]};
-    store_vec<T, 4>(p, t);
-}
+struct Eight {            // 8 elements as they lie
+    u32x4 r[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = reinterpret_cast<const u32x4*>(p)[i];
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 2) {
+            union { unsigned u; float f; } c;
+            const unsigned w = r[0][i >> 1];
+            c.u = i & 1 ? w & 0xffff0000u : w << 16;
+            return c.f;
+        } else {
+            union { unsigned u; float f; } c;
+            c.u = r[i >> 2][i & 3];
+            return c.f;
+        }
+    }
+};
 
 template <typename T, int ACT>
 struct EpiGate {          // h = act(a) u, and a | u where they are kept
     static constexpr bool GATED = true;
+    using Row = None;
+    struct Cols { float a[8], u[8]; };
     const T* bias;
     T* h;
     T* au;
     int F;
-    __device__ __forceinline__ void operator()(int m, int f, f32x4 a, f32x4 u) const {
+    __device__ __forceinline__ Cols columns(int f) const {
+        Cols c;
         if (bias) {
-            a += load4(bias + f);
-            u += load4(bias + F + f);
-        }
-        f32x4 r;
+            load_vec<T, 8>(bias + f, c.a);
+            load_vec<T, 8>(bias + F + f, c.u);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 8; ++e) c.a[e] = c.u[e] = 0.f;
+        }
+        return c;
+    }
+    __device__ __forceinline__ Row row(int, int) const { return Row{}; }
+    __device__ __forceinline__ void store(int m, int f, int, float (&a)[8], float (&u)[8], const Cols& c, const Row&) const {
+        float r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] += c.a[e];
+            u[e] += c.u[e];
             float v, d;
-            act_and_slope<ACT>(a[e], v, d);
+            act_and_slope<T, ACT>(a[e], v, d);
             r[e] = v * u[e];
         }
-        store4(h + (int64_t)m * F + f, r);
+        store_vec<T, 8>(h + (int64_t)m * F + f, r);
         if (au) {
-            store4(au + (int64_t)m * 2 * F + f, a);
-            store4(au + (int64_t)m * 2 * F + F + f, u);
+            store_vec<T, 8>(au + (int64_t)m * 2 * F + f, a);
+            store_vec<T, 8>(au + (int64_t)m * 2 * F + F + f, u);
         }
     }
 };
@@ -75,58 +111,99 @@ struct EpiGate {          // h = act(a) u, and a | u where they are kept
 template <typename T, int ACT>
 struct EpiGateBwd {       // dh -> da | du
     static constexpr bool GATED = false;
+    using Cols = None;
+    struct Row { Eight<T> a, u; };
     const T* au;
     T* dau;
     int F;
-    __device__ __forceinline__ void operator()(int m, int f, int, f32x4 dh) const {
-        const int64_t at = (int64_t)m * 2 * F + f;
-        const f32x4 a = load4(au + at), u = load4(au + at + F);
-        f32x4 da, du;
+    __device__ __forceinline__ Cols columns(int) const { return Cols{}; }
+    __device__ __forceinline__ Row row(int m, int f) const {
+        Row r;
+        r.a.load(au + (int64_t)m * 2 * F + f);
+        r.u.load(au + (int64_t)m * 2 * F + F + f);
+        return r;
+    }
+    __device__ __forceinline__ void store(int m, int f, int, float (&dh)[8], float (&)[8], const Cols&, const Row& r) const {
+        float da[8], du[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
             float v, d;
-            act_and_slope<ACT>(a[e], v, d);
-            da[e] = dh[e] * u[e] * d;
+            act_and_slope<T, ACT>(r.a[e], v, d);
+            da[e] = dh[e] * r.u[e] * d;
             du[e] = dh[e] * v;
         }
-        store4(dau + at, da);
-        store4(dau + at + F, du);
+        store_vec<T, 8>(dau + (int64_t)m * 2 * F + f, da);
+        store_vec<T, 8>(dau + (int64_t)m * 2 * F + F + f, du);
     }
 };
 
 template <typename T>
 struct EpiOut {           // bias, residual, one rounding
     static constexpr bool GATED = false;
+    struct Cols { float b[8]; };
+    struct Row { Eight<T> r; };
     const T* bias;
     const T* res;
     T* out;
     int64_t ldr, ldo;
-    __device__ __forceinline__ void operator()(int m, int n, int, f32x4 v) const {
-        if (bias) v += load4(bias + n);
-        if (res) v += load4(res + m * ldr + n);
-        store4(out + m * ldo + n, v);
+    __device__ __forceinline__ Cols columns(int n) const {
+        Cols c;
+        if (bias) {
+            load_vec<T, 8>(bias + n, c.b);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c.b[e] = 0.f;
+        }
+        return c;
+    }
+    __device__ __forceinline__ Row row(int m, int n) const {
+        Row r;
+        if (res) r.r.load(res + m * ldr + n);
+        return r;
+    }
+    __device__ __forceinline__ void store(int m, int n, int, float (&v)[8], float (&)[8], const Cols& c, const Row& r) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += c.b[e];
+        if (res) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r.r[e];
+        }
+        store_vec<T, 8>(out + m * ldo + n, v);
     }
 };
 
 struct EpiPart {          // one split's fp32 partial
     static constexpr bool GATED = false;
+    using Cols = None;
+    using Row = None;
     float* out;
     int64_t ld, split;
-    __device__ __forceinline__ void operator()(int m, int n, int sp, f32x4 v) const {
-        *reinterpret_cast<f32x4*>(out + sp * split + m * ld + n) = v;
+    __device__ __forceinline__ Cols columns(int) const { return Cols{}; }
+    __device__ __forceinline__ Row row(int, int) const { return Row{}; }
+    __device__ __forceinline__ void store(int m, int n, int sp, float (&v)[8], float (&)[8], const Cols&, const Row&) const {
+        store_vec<float, 8>(out + sp * split + m * ld + n, v);
     }
 };
 
-// the partials of a split product in split order, then the epilogue; 4 columns a thread
+// the partials of a split product in split order, then the epilogue; 8 columns a thread
 template <typename T>
 __global__ void __launch_bounds__(256) gemm_join_kernel(const float* part, int splits, int M, int N, const EpiOut<T> epi) {
-    const int64_t quads = (int64_t)M * (N / 4);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i / (N / 4)), n = (int)(i - (int64_t)m * (N / 4)) * 4;
+    const int64_t units = (int64_t)M * (N / 8);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < units; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i / (N / 8)), n = (int)(i - (int64_t)m * (N / 8)) * 8;
         const float* p = part + (int64_t)m * N + n;
-        f32x4 v = *reinterpret_cast<const f32x4*>(p);
-        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(p + s * (int64_t)M * N);
-        epi(m, n, 0, v);
+        const auto c = epi.columns(n);
+        const auto r = epi.row(m, n);
+        float v[8];
+        load_vec<float, 8>(p, v);
+#pragma unroll 4
+        for (int s = 1; s < splits; ++s) {
+            float t[8];
+            load_vec<float, 8>(p + s * (int64_t)M * N, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += t[e];
+        }
+        epi.store(m, n, 0, v, v, c, r);
     }
 }
 
@@ -237,8 +314,8 @@ static int run_gemm_out(const char* fn, const GemmSide<T>& x, const GemmSide<T>&
     NDB_REQUIRE(ws, fn, "workspace missing");
     const EpiPart part{ws, w.n, (int64_t)x.n * w.n};
     if (int rc = run_gemm<T, XK, WK>(fn, x, w, K, pl, 0, part, st)) return rc;
-    const int64_t quads = (int64_t)x.n * (w.n / 4);
-    const int64_t blocks = (quads + 255) / 256;
+    const int64_t units = (int64_t)x.n * (w.n / 8);
+    const int64_t blocks = (units + 255) / 256;
     hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, ws, pl.splits, x.n, w.n, epi);
     return check_launch(fn);
 }

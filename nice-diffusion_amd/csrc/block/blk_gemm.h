@@ -4,8 +4,8 @@
 // A workgroup of 4 waves (2 x 2) makes a tile of 64 TI x 64 TI outputs, a wave 32 TI x 32 TI: TI = 4 (256 x 256, one
 // workgroup a CU) or 2 (128 x 128, two).  Both operands go straight from memory to LDS (buffer loads with the LDS
 // destination, 16 bytes a lane) in two stages of 128 bytes of k; a wave reads one 16-byte piece a lane and k-step for each
-// of its 32-row fragments, 2 TI of them for TI^2 matrix instructions: LDS bandwidth is what a smaller wave tile would run
-// out of first.  The weights are the first operand of the matrix instruction, so a lane ends with 4 consecutive n of one m.
+// of its 32-row fragments, 2 TI of them for TI^2 matrix instructions.  The weights are the first operand of the matrix
+// instruction, so a lane ends with 4 consecutive n of one m.
 //
 //   LDS images   K-major: [row][8 pieces of 16 bytes], piece c of row r at c ^ (r >> 1 & 7): 16 rows read at one piece cover
 //                all 64 banks.  Otherwise [k][row], bf16 read back transposed (ds_read_b64_tr_b16: 4 k of 16 rows), piece c
@@ -14,9 +14,21 @@
 //   fp32 k-step  8 k:  lane half lh holds k = 4 lh + 0 .. 3; four v_mfma_f32_32x32x2_f32, each taking one k of either half.
 //   Loop         the fragments of a k-step are requested one step ahead; behind the last request of a stage one barrier
 //                hands that stage over to the loads of the tile after next, which then have a whole tile's time to arrive.
+//                With one wave a SIMD nothing else fills the matrix pipe, so every request sits between two matrix
+//                instructions (a fence after each keeps the compiler from gathering them).
 //   K tails      pieces past the end are made zero by the buffer range check (offset past the descriptor's size); rows past
 //                M or N hold whatever lies there inside the tensor, and their outputs are not stored.
+//   Epilogue     through LDS, 32 rows a wave at a time, so that a lane gets 8 consecutive n and a row's stores are whole lines.
+//
+// Measured, bf16 product alone at 16384 x 1024 x 8192 (275 GFLOP): 231 us K-major, 236 us with W [k][n] (1.19 / 1.16 PFLOP/s; the
+// library's product of 8192^3 runs at 1.39); 4096 x 4096 x 8192 with both [k][.] 216 us (1.27).  What bounds it: with the loads
+// taken out 189 us, the matrix instructions alone 137 us, the LDS reads alone 75 us (100 transposed), the loads alone 100 (rows of
+// 512 bytes) to 190 us (rows of 128): the LDS is written and read about two thirds of the time, which is what keeps the matrix pipe
+// from its rate.  Steps on the way, same product: requests in a bunch behind the barrier 282 us; 64-byte rows in a ring of 3, 4 or 5
+// stages 240 us, the depth making no difference; transposed reads that the compiler cannot tell from the loads in flight
+// (it then waits for them) 282 us.
 #pragma once
+#include <type_traits>
 #include "blk_common.h"
 
 namespace ndb {
@@ -63,14 +75,18 @@ struct GemmOperand {
     static constexpr int ROWB = TILE * ES;                   // not K-major: bytes of a k row
 
     unsigned off[NL];
-    int piece;                                               // K-major: k piece of the even loads; the odd ones have piece ^ 4
+    int piece;                                               // K-major: k piece of this lane's loads
     uint64_t base;
-    uint64_t left;                                           // bytes from base to the end of the tensor
-    int64_t step;                                            // bytes from one stage to the next
+    unsigned num;                                            // bytes that a whole stage may touch (descriptor size)
+    unsigned ldb, tailw;                                     // not K-major: bytes of a k row, and from the tile's first column to its end
+    unsigned soff;                                           // K-major: bytes along k
+    int64_t step;
     int frag0;
 
     __device__ __forceinline__ void init(const GemmSide<T>& s, int K, int row0, int k0, int wave, int lane, int wbase, int gate) {
-        const int64_t ldb = s.ld * ES;
+        const int64_t lb = s.ld * ES;
+        soff = 0;
+        ldb = (unsigned)lb;
         if constexpr (KMAJOR) {
             piece = (lane & 7) ^ (((lane >> 3) >> 1) & 7);
 #pragma unroll
@@ -81,13 +97,13 @@ struct GemmOperand {
                     const int wn = r8 / (32 * TI), in = r8 - wn * (32 * TI);
                     row = wn * (16 * TI) + (in & (16 * TI - 1)) + (in >= 16 * TI ? gate : 0) + (lane >> 3);
                 }
-                off[i] = (unsigned)(row * ldb) + (unsigned)((i & 1 ? piece ^ 4 : piece) << 4);
+                off[i] = (unsigned)(row * lb) + (unsigned)((i & 1 ? piece ^ 4 : piece) << 4);
             }
-            base = reinterpret_cast<uint64_t>(s.p) + (uint64_t)(row0 * ldb + (int64_t)k0 * ES);
-            left = (uint64_t)((s.n - 1 - row0) * ldb + (int64_t)(K - k0) * ES);
-            step = 128;
+            base = reinterpret_cast<uint64_t>(s.p) + (uint64_t)(row0 * lb + (int64_t)k0 * ES);
+            const uint64_t left = (uint64_t)((s.n - 1 - row0) * lb + (int64_t)(K - k0) * ES);
+            num = left < 0xfffffff0ull ? (unsigned)left : 0xfffffff0u;
             const int l31 = lane & 31, lh = lane >> 5;
-            frag0 = wbase * 128 + l31 * 128 + ((lh ^ ((l31 >> 1) & 7)) << 4);
+            frag0 = (wbase + l31) * 128 + ((lh ^ ((l31 >> 1) & 7)) << 4);
         } else {
             constexpr int CPR = ROWB / 16, RPL = 64 / CPR;   // pieces per k row, k rows per load
             static_assert(CPR <= 64, "a load covers whole k rows");
@@ -95,32 +111,33 @@ struct GemmOperand {
             for (int i = 0; i < NL; ++i) {
                 const int k = (wave * NL + i) * RPL + lane / CPR;
                 const int c = (lane & (CPR - 1)) ^ swz(k);
-                off[i] = (unsigned)(k * ldb) + (unsigned)(c << 4);
+                off[i] = (unsigned)(k * lb) + (unsigned)(c << 4);
             }
-            base = reinterpret_cast<uint64_t>(s.p) + (uint64_t)((int64_t)k0 * ldb + (int64_t)row0 * ES);
-            left = (uint64_t)((int64_t)(K - 1 - k0) * ldb + (int64_t)(s.n - row0) * ES);
-            step = (int64_t)KT * ldb;
+            base = reinterpret_cast<uint64_t>(s.p) + (uint64_t)((int64_t)k0 * lb + (int64_t)row0 * ES);
+            tailw = (unsigned)(s.n - row0) * ES;
+            num = (KT - 1) * ldb + tailw;
+            step = (int64_t)KT * lb;
             frag0 = wbase;
         }
     }
 
     static __device__ __forceinline__ int swz(int k) { return ES == 2 ? (k & 3) << 2 : ((k >> 2) & 1) << 3; }
 
-    // request a stage; krem: k left from this stage's first (K-major tails)
+    __device__ __forceinline__ void one(char* stage, int wave, int i, unsigned n, unsigned o) const {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, (int)n, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stage + (wave * NL + i) * 1024), 16, (int)o, (int)soff, 0, 0);
+    }
+    __device__ __forceinline__ void advance() {
+        if constexpr (KMAJOR) soff += 128;
+        else base += (uint64_t)step;
+    }
+    // request a stage of which krem >= 1 k are left
     __device__ __forceinline__ void load(char* stage, int wave, int krem) {
-        const uint64_t cap = left < 0xfffffff0ull ? left : 0xfffffff0ull;
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, (int)(unsigned)cap, 0x00020000);
+        unsigned n = num;
+        if (!KMAJOR && krem < KT) n = (unsigned)(krem - 1) * ldb + tailw;
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            unsigned o = off[i];
-            if (KMAJOR && krem < KT) {
-                const int pc = i & 1 ? piece ^ 4 : piece;
-                o = pc * PIECE < krem ? o : 0xfffffff0u;
-            }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stage + (wave * NL + i) * 1024), 16, (int)o, 0, 0, 0);
-        }
-        base += (uint64_t)step;
-        left = left > (uint64_t)step ? left - (uint64_t)step : 0;
+        for (int i = 0; i < NL; ++i) one(stage, wave, i, n, KMAJOR && (i & 1 ? piece ^ 4 : piece) * PIECE >= krem ? 0xfffffff0u : off[i]);
+        advance();
     }
 
     // 16 bytes a lane: row wbase + 32 t + l31, k-step s (lane half lh)
@@ -157,6 +174,66 @@ struct GemmOperand {
 template <int TI>
 constexpr int gemm_lds_bytes() { return 2 * 2 * 64 * TI * 128; }
 
+#define NDB_SB __builtin_amdgcn_sched_barrier(0x6)
+// one k-step of a stage: the matrix instructions of fragments c, and between them the fragments of the next step from `src` and
+// (REQ) the requests of a whole stage into `dst`
+template <typename T, int TI, class X, class W, int c, int s, bool REQ>
+__device__ __forceinline__ void gemm_step(const char* src, char* dst, const X& x, const W& w, u32x4 (&fx)[2][TI], u32x4 (&fw)[2][TI], f32x16 (&acc)[TI][TI], int wave, int lane) {
+    constexpr int SZ = X::STAGE, PER = X::NL + W::NL;
+#pragma unroll
+    for (int a = 0; a < TI; ++a)
+#pragma unroll
+        for (int b = 0; b < TI; ++b) {
+            acc[a][b] = mma_step<T>(fw[c][a], fx[c][b], acc[a][b]);
+            NDB_SB;
+            const int i = a * TI + b;
+            if (i < TI) fw[c ^ 1][i] = w.frag(src + SZ, lane, i, s);
+            else if (i < 2 * TI) fx[c ^ 1][i - TI] = x.frag(src, lane, i - TI, s);
+            if (REQ) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    if ((TI == 4 ? j : j / 2) != i) continue;          // PER = TI^2 of them at TI = 4, 2 TI^2 at 2
+                    if (j < X::NL) x.one(dst, wave, j, x.num, x.off[j % X::NL]);
+                    else w.one(dst + SZ, wave, j - X::NL, w.num, w.off[(j - X::NL) % W::NL]);
+                }
+            }
+            NDB_SB;
+        }
+}
+// every read of this stage has returned and the next stage has landed, in all waves
+__device__ __forceinline__ void gemm_sync() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070);                       // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// Whole stages with a whole stage to request, two at a time; returns how many.  The stages are restrict pointers: the compiler
+// then knows that the fragments it reads are not those that a load in flight will write, and does not wait for it.
+template <typename T, int TI, class X, class W>
+__device__ __forceinline__ int gemm_loop(char* __restrict__ sa, char* __restrict__ sb, X& x, W& w, u32x4 (&fx)[2][TI], u32x4 (&fw)[2][TI], f32x16 (&acc)[TI][TI], int end, int wave, int lane) {
+    int kt = 0;
+    for (; kt + 1 < end; kt += 2) {
+        gemm_step<T, TI, X, W, 0, 1, false>(sa, sa, x, w, fx, fw, acc, wave, lane);
+        gemm_step<T, TI, X, W, 1, 2, false>(sa, sa, x, w, fx, fw, acc, wave, lane);
+        gemm_step<T, TI, X, W, 0, 3, false>(sa, sa, x, w, fx, fw, acc, wave, lane);
+        gemm_sync();
+        gemm_step<T, TI, X, W, 1, 0, true>(sb, sa, x, w, fx, fw, acc, wave, lane);
+        x.advance();
+        w.advance();
+        gemm_step<T, TI, X, W, 0, 1, false>(sb, sb, x, w, fx, fw, acc, wave, lane);
+        gemm_step<T, TI, X, W, 1, 2, false>(sb, sb, x, w, fx, fw, acc, wave, lane);
+        gemm_step<T, TI, X, W, 0, 3, false>(sb, sb, x, w, fx, fw, acc, wave, lane);
+        gemm_sync();
+        gemm_step<T, TI, X, W, 1, 0, true>(sa, sb, x, w, fx, fw, acc, wave, lane);
+        x.advance();
+        w.advance();
+    }
+    return kt;
+}
+#undef NDB_SB
+
 template <typename T, int TI, bool XK, bool WK, class Epi>
 __global__ void __launch_bounds__(GEMM_THREADS, TI == 4 ? 1 : 2) gemm_kernel(const GemmArgs<T> p, const Epi epi) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -184,54 +261,49 @@ __global__ void __launch_bounds__(GEMM_THREADS, TI == 4 ? 1 : 2) gemm_kernel(con
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
 
-    char* const sx[2] = {smem, smem + SZ};
-    char* const sw[2] = {smem + 2 * SZ, smem + 3 * SZ};
-    x.load(sx[0], wave, p.K - k0);
-    w.load(sw[0], wave, p.K - k0);
-    asm volatile("" ::: "memory");          // the count below tells the two stages' loads apart by their order
+    auto ax = [&](int st) { return smem + st * 2 * SZ; };
+    constexpr int PER = X::NL + W::NL;
+    x.load(ax(0), wave, p.K - k0);
+    w.load(ax(0) + SZ, wave, p.K - k0);
+    asm volatile("" ::: "memory");
     if (nt > 1) {
-        x.load(sx[1], wave, p.K - k0 - KT);
-        w.load(sw[1], wave, p.K - k0 - KT);
+        x.load(ax(1), wave, p.K - k0 - KT);
+        w.load(ax(1) + SZ, wave, p.K - k0 - KT);
     }
     u32x4 fx[2][TI], fw[2][TI];
-    if (nt > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(X::NL + W::NL) : "memory");
+    if (nt > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int t = 0; t < TI; ++t) {
-        fx[0][t] = x.frag(sx[0], lane, t, 0);
-        fw[0][t] = w.frag(sw[0], lane, t, 0);
+        fx[0][t] = x.frag(ax(0), lane, t, 0);
+        fw[0][t] = w.frag(ax(0) + SZ, lane, t, 0);
     }
-    for (int kt = 0; kt < nt; ++kt) {
-        const int cur = kt & 1;
-        char* const cx = smem + cur * SZ;
-        char* const cw = smem + 2 * SZ + cur * SZ;
-        char* const nx = smem + (cur ^ 1) * SZ;
-        char* const nw = smem + 2 * SZ + (cur ^ 1) * SZ;
+    int kt = gemm_loop<T, TI, X, W>(ax(0), ax(1), x, w, fx, fw, acc, nt - ((p.K - k0) % KT ? 3 : 2), wave, lane);
+    for (; kt < nt; ++kt) {          // the last few: nothing or a cut stage to request
+        char* const cs = ax(kt & 1);
+        char* const ns = ax((kt & 1) ^ 1);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const int c = s & 1, n = c ^ 1;
+            const int c = s & 1;
             if (s < 3) {
 #pragma unroll
                 for (int t = 0; t < TI; ++t) {
-                    fx[n][t] = x.frag(cx, lane, t, s + 1);
-                    fw[n][t] = w.frag(cw, lane, t, s + 1);
+                    fx[c ^ 1][t] = x.frag(cs, lane, t, s + 1);
+                    fw[c ^ 1][t] = w.frag(cs + SZ, lane, t, s + 1);
                 }
             } else if (kt + 1 < nt) {
-                // every read of this stage has returned and the next stage has landed, in all waves
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
+                gemm_sync();
                 if (kt + 2 < nt) {
                     const int krem = p.K - k0 - (kt + 2) * KT;
-                    x.load(cx, wave, krem);
-                    w.load(cw, wave, krem);
+                    x.load(cs, wave, krem);
+                    w.load(cs + SZ, wave, krem);
                 }
 #pragma unroll
                 for (int t = 0; t < TI; ++t) {
-                    fx[n][t] = x.frag(nx, lane, t, 0);
-                    fw[n][t] = w.frag(nw, lane, t, 0);
+                    fx[c ^ 1][t] = x.frag(ns, lane, t, 0);
+                    fw[c ^ 1][t] = w.frag(ns + SZ, lane, t, 0);
                 }
             }
 #pragma unroll
@@ -240,32 +312,43 @@ __global__ void __launch_bounds__(GEMM_THREADS, TI == 4 ? 1 : 2) gemm_kernel(con
                 for (int b = 0; b < TI; ++b) acc[a][b] = mma_step<T>(fw[c][a], fx[c][b], acc[a][b]);
         }
     }
-    // a lane's piece: row m, columns n .. n + 3
-    const int l31 = lane & 31, lh = lane >> 5;
+    __builtin_amdgcn_s_barrier();                             // every wave is through with the stages
+    asm volatile("" ::: "memory");
+    // 32 rows at a time: registers -> LDS [row][32 TI fp32, pieces of 4 at piece ^ row] -> 8 consecutive n a lane
+    constexpr int PPR = 8 * TI, LPR = Epi::GATED ? 2 * TI : 4 * TI, RPI = 64 / LPR, NIT = 32 / RPI;
+    const int l31 = lane & 31, lh = lane >> 5, col = lane & (LPR - 1);
+    char* const mine = smem + wave * (32 * 32 * TI * 4);
+    const int n = Epi::GATED ? n0 + wn * 16 * TI + col * 8 : n0 + wn * 32 * TI + col * 8;
+    const bool n_in = n < (Epi::GATED ? p.gate_rows : p.w.n);
+    const auto cols = epi.columns(n_in ? n : 0);
+    auto piece_at = [&](int r, int c) { return reinterpret_cast<f32x4*>(mine + r * (128 * TI) + ((c ^ (r & (PPR - 1))) << 4)); };
 #pragma unroll
     for (int b = 0; b < TI; ++b) {
-        const int m = m0 + wm * 32 * TI + b * 32 + l31;
-        if (m >= p.x.n) continue;
-        if constexpr (Epi::GATED) {
+        const int mb = m0 + wm * 32 * TI + b * 32;
+        typename Epi::Row extra[NIT];
 #pragma unroll
-            for (int a = 0; a < TI / 2; ++a)
+        for (int it = 0; it < NIT; ++it) {
+            const int m = mb + it * RPI + lane / LPR;
+            if (n_in && m < p.x.n) extra[it] = epi.row(m, n);
+        }
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int f = n0 + wn * 16 * TI + a * 32 + 8 * g + 4 * lh;
-                    const f32x4 u = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
-                    const f32x4 v = {acc[a + TI / 2][b][4 * g], acc[a + TI / 2][b][4 * g + 1], acc[a + TI / 2][b][4 * g + 2],
-                                     acc[a + TI / 2][b][4 * g + 3]};
-                    if (f < p.gate_rows) epi(m, f, u, v);
-                }
-        } else {
+        for (int a = 0; a < TI; ++a)
 #pragma unroll
-            for (int a = 0; a < TI; ++a)
+            for (int g = 0; g < 4; ++g)
+                *piece_at(l31, a * 8 + 2 * g + lh) = f32x4{acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int n = n0 + wn * 32 * TI + a * 32 + 8 * g + 4 * lh;
-                    const f32x4 u = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
-                    if (n < p.w.n) epi(m, n, sp, u);
-                }
+        for (int it = 0; it < NIT; ++it) {
+            const int r = it * RPI + lane / LPR, m = mb + r;
+            float v[8], u[8];
+            const f32x4 v0 = *piece_at(r, 2 * col), v1 = *piece_at(r, 2 * col + 1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = v0[e], v[4 + e] = v1[e];
+            if constexpr (Epi::GATED) {
+                const f32x4 u0 = *piece_at(r, PPR / 2 + 2 * col), u1 = *piece_at(r, PPR / 2 + 2 * col + 1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = u0[e], u[4 + e] = u1[e];
+            }
+            if (n_in && m < p.x.n) epi.store(m, n, sp, v, u, cols, extra[it]);
         }
     }
 }
