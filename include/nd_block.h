@@ -70,7 +70,7 @@ int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_s
                           int64_t do_sh, void* dq, void* dk, void* dv, void* dlambda_q1, void* dlambda_k1, void* dlambda_q2,
                           void* dlambda_k2, float* workspace, int B, int Tq, int Tk, int H, int Hk, int D, int Dv, float scale, int flags,
                           int dtype, nd_stream_t stream);
-int64_t nd_diff_attention_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hk);
+int64_t nd_diff_attention_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int dtype);
 
 /* ---- gated feed-forward block ----------------------------------------------------------------------------------------- */
 

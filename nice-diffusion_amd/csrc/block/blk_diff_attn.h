@@ -24,8 +24,8 @@ struct Tile {
         return *reinterpret_cast<const u32x4*>(t + (base ^ ((c & 15) << 4)) + (c >> 4) * 256 + r0 * RB);
     }
 
-    // columns: bf16 cols(): lane (d = col + l31) gets rows r0 + 4 lh + 0 .. 3 and r0 + 8 + 4 lh + 0 .. 3 (the k order in which an
-    // accumulator's registers serve as the other operand); fp32 one(): row r0 + (e & 3) + 8 (e >> 2) + 4 lh.  col a multiple of
+    // columns: bf16 cols2(): lane (d = col + l31) gets, of k-step s, rows r0 + 16 s + 4 lh + 0 .. 3 and 8 further (the k order in
+    // which an accumulator's registers serve as the other operand); fp32 one(): row r0 + (e & 3) + 8 (e >> 2) + 4 lh.  col a multiple of
     // 32, r0 of 16 (bf16) / 32.
     static __device__ __forceinline__ int col_base(int lane) {
         const int lh = lane >> 5;
@@ -35,16 +35,39 @@ struct Tile {
         }
         return 4 * lh * RB + ((((lane & 31) >> 2) ^ swz(4 * lh)) << 4) + (lane & 3) * 4;
     }
-    static __device__ __forceinline__ u32x4 cols(const char* t, int base, int r0, int col) {
-        u32x4 v;
+    // the fragments of two 32-column blocks col, col + 32 for rows r0 .. r0 + 31: f[block][k-step].  Eight transposed reads and their
+    // wait in one piece of assembly: of the builtin the compiler believes that it may read what a load in flight to the other
+    // stage writes, and waits for that load.
+    static __device__ __forceinline__ void cols2(const char* t, int base, int r0, int col, u32x4 (&f)[2][2]) {
+        const int at = (int)(uintptr_t)(__attribute__((address_space(3))) const char*)t + r0 * RB;
+        u32x2 v[2][2][2];          // [block][k-step][rows + 8]
+        const int a0 = at + (base ^ ((col / 8 & 15) << 4)), a1 = at + (base ^ (((col / 8 & 15) ^ 2) << 4));
+        const int b0 = at + (base ^ (((col + 32) / 8 & 15) << 4)), b1 = at + (base ^ ((((col + 32) / 8 & 15) ^ 2) << 4));
+        const int ca = (col / 128) * 256, cb = ((col + 32) / 128) * 256;
+        static_assert(24 * RB + 512 < 65536, "offsets fit the instruction");
+        if (ca == 0 && cb == 0) cols2_asm<0, 0>(v, a0, a1, b0, b1);
+        else cols2_asm<256, 256>(v, a0, a1, b0, b1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const char* a = t + (base ^ (((col / 8 & 15) ^ (2 * h)) << 4)) + (col / 128) * 256 + (r0 + 8 * h) * RB;
-            union { s16x4 h4; unsigned u[2]; } c;
-            c.h4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
-            v[2 * h] = c.u[0], v[2 * h + 1] = c.u[1];
-        }
-        return v;
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) f[d][s] = u32x4{v[d][s][0][0], v[d][s][0][1], v[d][s][1][0], v[d][s][1][1]};
+    }
+    template <int CA, int CB>
+    static __device__ __forceinline__ void cols2_asm(u32x2 (&v)[2][2][2], int a0, int a1, int b0, int b1) {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %1, %9 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %2, %8 offset:%14\n\t"
+            "ds_read_b64_tr_b16 %3, %9 offset:%15\n\t"
+            "ds_read_b64_tr_b16 %4, %10 offset:%16\n\t"
+            "ds_read_b64_tr_b16 %5, %11 offset:%17\n\t"
+            "ds_read_b64_tr_b16 %6, %10 offset:%18\n\t"
+            "ds_read_b64_tr_b16 %7, %11 offset:%19\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(v[0][0][0]), "=&v"(v[0][0][1]), "=&v"(v[0][1][0]), "=&v"(v[0][1][1]), "=&v"(v[1][0][0]), "=&v"(v[1][0][1]),
+              "=&v"(v[1][1][0]), "=&v"(v[1][1][1])
+            : "v"(a0), "v"(a1), "v"(b0), "v"(b1), "n"(CA), "n"(CA + 8 * RB), "n"(CA + 16 * RB), "n"(CA + 24 * RB), "n"(CB),
+              "n"(CB + 8 * RB), "n"(CB + 16 * RB), "n"(CB + 24 * RB));
     }
     static __device__ __forceinline__ float one(const char* t, int base, int r0, int e, int col) {
         const int r = (e & 3) + 8 * (e >> 2);
@@ -56,6 +79,24 @@ struct Tile {
 __device__ __forceinline__ int in_loop(int v) {
     asm volatile("" : "+v"(v));
     return v;
+}
+
+// over the two lanes (halves) that hold a column of an accumulator
+__device__ __forceinline__ float half_max(float v) {
+    union { float f; unsigned u; } x;
+    x.f = v;
+    const auto r = __builtin_amdgcn_permlane32_swap(x.u, x.u, false, false);
+    union { unsigned u; float f; } a, b;
+    a.u = r[0], b.u = r[1];
+    return fmaxf(a.f, b.f);
+}
+__device__ __forceinline__ float half_sum(float v) {
+    union { float f; unsigned u; } x;
+    x.f = v;
+    const auto r = __builtin_amdgcn_permlane32_swap(x.u, x.u, false, false);
+    union { unsigned u; float f; } a, b;
+    a.u = r[0], b.u = r[1];
+    return a.f + b.f;
 }
 
 // this wave's share of filling such a tile
@@ -115,21 +156,50 @@ struct Probs<float> {
     }
 };
 
-// acc[d][column] += sum over the 32 rows r0 .. of tile[row][col0 + d] * p[row][column]
-template <typename T, int RB>
-__device__ __forceinline__ f32x16 mma_cols(const char* t, int base, int r0, int col, const Probs<T>& p, f32x16 acc) {
+// acc[n][d][column] += sum over the 32 rows r0 .. of tile[row][col + 32 n + d] * p[row][column], for N blocks of columns
+template <typename T, int RB, int N>
+__device__ __forceinline__ void mma_cols(const char* t, int base, int r0, int col, const Probs<T>& p, f32x16 (&acc)[N]) {
     if constexpr (sizeof(T) == 2) {
+        static_assert(N % 2 == 0, "blocks in pairs");
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            union { u32x4 u; bf16x8 h; } a;
-            a.u = Tile<T, RB>::cols(t, base, r0 + 16 * s, col);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, p.f[s], acc, 0, 0, 0);
+        for (int n = 0; n < N; n += 2) {
+            u32x4 f[2][2];
+            Tile<T, RB>::cols2(t, base, r0, col + 32 * n, f);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    union { u32x4 u; bf16x8 h; } a;
+                    a.u = f[i][s];
+                    acc[n + i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, p.f[s], acc[n + i], 0, 0, 0);
+                }
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Tile<T, RB>::one(t, base, r0, e, col), p.f[e], acc, 0, 0, 0);
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(Tile<T, RB>::one(t, base, r0, e, col + 32 * n), p.f[e], acc[n], 0, 0, 0);
     }
-    return acc;
+}
+
+// both maps' products with the halves of one tile: acc[m][d][column] += sum over rows of tile[row][m HD + 32 d ..] * p[m][row][column]
+template <typename T, int RB, int HD>
+__device__ __forceinline__ void mma_halves(const char* t, int base, const Probs<T>& p0, const Probs<T>& p1, f32x16 (&acc)[2][HD / 32]) {
+    if constexpr (sizeof(T) == 2 && HD == 32) {              // one block of each half: a pair
+        u32x4 f[2][2];
+        Tile<T, RB>::cols2(t, base, 0, 0, f);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            union { u32x4 u; bf16x8 h; } a, b;
+            a.u = f[0][s], b.u = f[1][s];
+            acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, p0.f[s], acc[0][0], 0, 0, 0);
+            acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b.h, p1.f[s], acc[1][0], 0, 0, 0);
+        }
+    } else {
+        mma_cols<T, RB>(t, base, 0, 0, p0, acc[0]);
+        mma_cols<T, RB>(t, base, 0, HD, p1, acc[1]);
+    }
 }
 
 struct DiffTensor {       // [batch, token, head, channel], channels contiguous
@@ -179,12 +249,51 @@ __device__ __forceinline__ void diff_lambda(const DiffArgs& p, int head, int lan
     e2 = expf(b);
 }
 
+// A ring of NST stages: fetch(i, stage) requests tile i (PER vector-memory operations a wave, always as many), NST - 1 tiles ahead
+// of compute(i, stage).  Other such operations in between only make the wait for a tile stricter.
+template <int NST, int PER, class Fetch, class Compute>
+__device__ __forceinline__ void ring(char* stages, int bytes, int n, Fetch&& fetch, Compute&& compute) {
+    static_assert((NST - 2) * PER < 64, "the counter's range");
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+        if (i < n) fetch(i, stages + i * bytes);
+    int now = 0;
+    for (int i = 0; i < n; ++i) {
+        // tile i has landed (the NST - 2 behind it may be under way) ...
+        if (i + NST - 1 <= n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * PER) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                         // ... in all waves, and they are through with tile i - 1
+        asm volatile("" ::: "memory");
+        if (i + NST - 1 < n) fetch(i + NST - 1, stages + (now == 0 ? NST - 1 : now - 1) * bytes);
+        compute(i, stages + now * bytes);
+        now = now + 1 == NST ? 0 : now + 1;
+    }
+}
+
 constexpr int DIFF_MAX_GROUP = 64;
 
 // consecutive workgroup ids go to the 8 XCDs in turn: give each a contiguous run, so that the readers of one head's keys share an L2
 __device__ __forceinline__ int xcd_run(int lin, int total) {
     const int q = total >> 3, r = total & 7, x = lin & 7;
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (lin >> 3);
+}
+
+// workgroup -> (batch and key head, index within).  Consecutive ids go to the 8 XCDs in turn; each XCD gets whole (batch, key head)s,
+// whose readers then share an L2.  Units of equal length: one after the other.  Causal ones (index 0 the longest): the longest
+// of all of them first, so that the short ones fill the end.
+__device__ __forceinline__ void unit_of(int lin, int total, int units, int causal, int& unit, int& index) {
+    if (causal && units % 8 == 0) {
+        const int per = units >> 3, j = lin >> 3;
+        index = j / per;
+        unit = (lin & 7) * per + j - index * per;
+    } else if (causal) {
+        index = lin / units;
+        unit = lin - index * units;
+    } else {
+        const int id = xcd_run(lin, total), per = total / units;
+        unit = id / per;
+        index = id - unit * per;
+    }
 }
 
 }  // namespace ndb

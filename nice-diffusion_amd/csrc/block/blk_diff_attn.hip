@@ -15,8 +15,9 @@
 //              queries of 256 channels do not fit the registers (measured: 290 spilled)
 //   splits     when (batch, key head, row tile) does not fill the chip the keys are divided over workgroups; fp32 partial
 //              outputs, joined in split order by a second launch
-// The maximum a row is scaled by only moves when a score exceeds it by 2^8 (p <= 256: as exact in floating point).  Rounding to
-// bf16 besides the output: the weights p as the second product's operand; their sum is taken from the rounded values.
+// No maximum is taken of a tile as a rule: its weights are made against the row's reference of before, and only where their sum
+// passes 2^10 (or nothing was seen so far) the reference moves to the tile's maximum and they are made again: a weight stays
+// below 2^10, as exact in floating point as one below 1.  Rounding to bf16 besides the output: the weights p as the second product's operand; their sum is taken from the rounded values.
 #include "blk_diff_attn.h"
 
 namespace ndb {
@@ -29,41 +30,34 @@ struct DiffShape {
     static constexpr int NS = PH / 2;                        // steps of a score product
     static constexpr int NDT = DV / 32;
     static constexpr int KT_MANY = (ES == 4 && HD == 128) ? 32 : 64;
-    static constexpr int KT_FEW = 128 * (RBK + RBV) <= 65536 ? 128 : (64 * (RBK + RBV) <= 65536 ? 64 : 32);
+    static constexpr int KT_FEW = 128 * (RBK + RBV) <= 32768 ? 128 : (64 * (RBK + RBV) <= 32768 ? 64 : 32);     // two workgroups a CU
 };
-
-template <typename T, int HD, bool FEW>
-constexpr int diff_lds_bytes() {
-    using S = DiffShape<T, HD>;
-    constexpr int kt = FEW ? S::KT_FEW : S::KT_MANY, stages = 2 * kt * (S::RBK + S::RBV);
-    constexpr int join = FEW ? 32 * (2 * S::DV + 4) * 4 + (S::KT_FEW / 32) * 32 * 16 : 0;
-    return (stages > join ? stages : join) + DIFF_MAX_GROUP * 4;
-}
 
 template <typename T, int HD, bool FEW>
 constexpr int diff_threads() { return FEW ? 2 * DiffShape<T, HD>::KT_FEW : 256; }
 
 template <typename T, int HD, bool FEW>
-__global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeof(T) >= 256 ? 1 : 2)) diff_attn_kernel(const DiffArgs p) {
+__global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeof(T) >= 256 ? 1 : (HD == 32 && sizeof(T) == 2 && !FEW ? 3 : 2))) diff_attn_kernel(const DiffArgs p) {
     using S = DiffShape<T, HD>;
     constexpr int KT = FEW ? S::KT_FEW : S::KT_MANY;
     constexpr int NW = FEW ? KT / 32 : 4;                    // waves
+    constexpr int NJ = 1;                                     // 32-key blocks at a time (2 at D <= 32: 181 registers for 142, no faster)
     constexpr int STAGE = KT * (S::RBK + S::RBV);
+    constexpr int NST = !FEW && HD == 32 && S::ES == 2 ? 3 : 2;                      // tiles in LDS
     using TK = Tile<T, S::RBK>;
     using TV = Tile<T, S::RBV>;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* const lam_s = reinterpret_cast<float*>(smem + diff_lds_bytes<T, HD, FEW>() - DIFF_MAX_GROUP * 4);
+    static_assert(!FEW || NW == 1 || NW * 32 * 16 + 32 * (2 * S::DV + 4) * 4 <= NST * STAGE, "the waves' join fits the stages");
+    __shared__ __attribute__((aligned(16))) char stages[NST * STAGE];
+    __shared__ float lam_s[DIFF_MAX_GROUP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, lh = lane >> 5;
 
     const int rows = p.Tq * p.g, tiles = (rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
-    const int vblocks = (p.Dv + S::DV - 1) / S::DV;
-    int id = xcd_run(blockIdx.x, gridDim.x);
-    const int per = tiles * p.splits * vblocks, bh = id / per;
-    id -= bh * per;
+    int bh, id;
+    unit_of(blockIdx.x, gridDim.x, p.B * p.Hk, p.causal, bh, id);
     const int vb = HD == 128 ? id / (tiles * p.splits) : 0, dv0 = vb * S::DV, dvn = p.Dv - dv0 < S::DV ? p.Dv - dv0 : S::DV;
     id -= vb * tiles * p.splits;
-    const int sp = id / tiles, tile = p.causal ? tiles - 1 - (id - sp * tiles) : id - sp * tiles;      // causal: longest rows first
+    const int sp = id / tiles, tile = tiles - 1 - (id - sp * tiles);      // longest rows first
     const int b = bh / p.Hk, hk = bh - b * p.Hk;
     const int len = diff_length(p.lengths, b, p.Tk);
 
@@ -113,55 +107,70 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
     lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, wave, lane);
     const T* kp = static_cast<const T*>(p.k.p) + b * p.k.sb + hk * p.k.sh;
     const T* vp = static_cast<const T*>(p.v.p) + b * p.v.sb + hk * p.v.sh + dv0;
-    auto fetch = [&](int key, int stage) {                    // keys at or past the sequence's end become zero rows
-        char* at = smem + stage * STAGE;
+    auto fetch = [&](int i, char* at) {                       // keys at or past the sequence's end become zero rows
+        const int key = kbeg + i * KT;
         const int64_t n = len - key;
         lk.load(at, kp + (int64_t)key * p.k.st, ((n - 1) * p.k.st + 2 * p.D) * S::ES, wave);
         lv.load(at + KT * S::RBK, vp + (int64_t)key * p.v.st, ((n - 1) * p.v.st + dvn) * S::ES, wave);
     };
     const int row_base = TK::row_base(lane), col_base = TV::col_base(lane);
-    if (kbeg < kend) fetch(kbeg, 0);
-    int stage = 0;
-    for (int key0 = kbeg; key0 < kend; key0 += KT, stage ^= 1) {
-        // this stage has landed, and every wave is through with the other one
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (key0 + KT < kend) fetch(key0 + KT, stage ^ 1);
-        const char* tk = smem + stage * STAGE;
+    auto compute = [&](int i, const char* tk) {
+        const int key0 = kbeg + i * KT;
         const char* tv = tk + KT * S::RBK;
 #pragma unroll 1
-        for (int sub = FEW ? wave : 0; sub < (FEW ? wave + 1 : KT / 32); ++sub) {
+        for (int sub = FEW ? wave : 0; sub < (FEW ? wave + 1 : KT / 32); sub += NJ) {
             const int kb = key0 + sub * 32;
             if (kb >= kend) break;
-            const int rb = in_loop(row_base), cb = in_loop(col_base), r32 = sub * 32;
-            f32x16 s[2];
+            const int rb = in_loop(row_base), cb = in_loop(col_base);
+            const char* k32 = tk + sub * 32 * S::RBK;
+            const char* v32 = tv + sub * 32 * S::RBV;
+            f32x16 s[2][NJ];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[m][e] = 0.f;
+                for (int m = 0; m < 2; ++m) {
 #pragma unroll
-                for (int c = 0; c < S::NS; ++c) s[m] = mma_step<T>(TK::row(tk + r32 * S::RBK, rb, 0, m * S::PH + 2 * c), q[m][c], s[m]);
-            }
+                    for (int e = 0; e < 16; ++e) s[m][j][e] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < S::NS; ++c) s[m][j] = mma_step<T>(TK::row(k32, rb, 32 * j, m * S::PH + 2 * c), q[m][c], s[m][j]);
+                }
             // scores past what a row sees: only in the tile that holds a row's end
-            const bool cut = p.causal ? kb + 32 > r0 / p.g + len - p.Tq + 1 : kb + 32 > len;
+            const bool cut = p.causal ? kb + 32 * NJ > r0 / p.g + len - p.Tq + 1 : kb + 32 * NJ > len;
             if (cut) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const bool in = kb + (e & 3) + 8 * (e >> 2) + 4 * lh < seen;
-                    s[0][e] = in ? s[0][e] : -INFINITY;
-                    s[1][e] = in ? s[1][e] : -INFINITY;
-                }
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const bool in = kb + 32 * j + (e & 3) + 8 * (e >> 2) + 4 * lh < seen;
+                        s[0][j][e] = in ? s[0][j][e] : -INFINITY;
+                        s[1][j][e] = in ? s[1][j][e] : -INFINITY;
+                    }
             }
-            Probs<T> pr[2];
+            Probs<T> pr[2][NJ];
+            float sum[2];
+            auto weights = [&](int m) {                       // sum: this lane half's keys; the halves meet at the end
+                const float ref = mx[m] == -INFINITY ? 0.f : mx[m];
+                sum[m] = 0.f;
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                float top = fmaxf(s[m][0], s[m][1]);
+                for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-                for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(s[m][e], s[m][e + 1]), top);
-                top = fmaxf(top, __shfl_xor(top, 32)) * p.c;
-                const bool move = top > mx[m] + 8.f;          // also from -inf
-                if (__builtin_amdgcn_ballot_w64(move) != 0) {
+                    for (int e = 0; e < 16; ++e) pr[m][j].set(e, __builtin_amdgcn_exp2f(fmaf(s[m][j][e], p.c, -ref)));
+                    sum[m] += pr[m][j].sum();
+                }
+            };
+            weights(0);
+            weights(1);
+            const bool again = mx[0] == -INFINITY || mx[1] == -INFINITY || fmaxf(sum[0], sum[1]) > 1024.f;
+            if (__builtin_amdgcn_ballot_w64(again) != 0) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(s[m][j][e], s[m][j][e + 1]), top);
+                    top = half_max(top) * p.c;
+                    const bool move = top > mx[m];
                     const float a = move ? __builtin_amdgcn_exp2f(mx[m] - top) : 1.f;
                     mx[m] = move ? top : mx[m];
                     l[m] *= a;
@@ -169,40 +178,50 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
                     for (int d = 0; d < S::NDT; ++d)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[m][d][e] *= a;
+                    weights(m);
                 }
-                const float ref = mx[m] == -INFINITY ? 0.f : mx[m];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) pr[m].set(e, __builtin_amdgcn_exp2f(fmaf(s[m][e], p.c, -ref)));
-                l[m] += pr[m].sum();                          // this lane half's keys; the halves meet at the end
             }
+            l[0] += sum[0];
+            l[1] += sum[1];
 #pragma unroll
-            for (int d = 0; d < S::NDT; ++d) {
+            for (int j = 0; j < NJ; ++j) {
                 if constexpr (S::ES == 2) {
 #pragma unroll
-                    for (int s2 = 0; s2 < 2; ++s2) {
-                        union { u32x4 u; bf16x8 h; } a;
-                        a.u = TV::cols(tv + r32 * S::RBV, cb, 16 * s2, d * 32);
-                        o[0][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, pr[0].f[s2], o[0][d], 0, 0, 0);
-                        o[1][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, pr[1].f[s2], o[1][d], 0, 0, 0);
+                    for (int d = 0; d < S::NDT; d += 2) {     // the value fragments serve both maps
+                        u32x4 f[2][2];
+                        TV::cols2(v32, cb, 32 * j, d * 32, f);
+#pragma unroll
+                        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) {
+                                    union { u32x4 u; bf16x8 h; } a;
+                                    a.u = f[x][s2];
+                                    o[m][d + x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, pr[m][j].f[s2], o[m][d + x], 0, 0, 0);
+                                }
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float a = TV::one(tv + r32 * S::RBV, cb, 0, e, d * 32);
-                        o[0][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[0].f[e], o[0][d], 0, 0, 0);
-                        o[1][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[1].f[e], o[1][d], 0, 0, 0);
-                    }
+                    for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float a = TV::one(v32, cb, 32 * j, e, d * 32);
+                            o[0][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[0][j].f[e], o[0][d], 0, 0, 0);
+                            o[1][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[1][j].f[e], o[1][d], 0, 0, 0);
+                        }
                 }
             }
         }
-    }
-    l[0] += __shfl_xor(l[0], 32);
-    l[1] += __shfl_xor(l[1], 32);
+    };
+    ring<NST, decltype(lk)::NI + decltype(lv)::NI>(stages, STAGE, kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0, fetch, compute);
+    l[0] = half_sum(l[0]);
+    l[1] = half_sum(l[1]);
     __syncthreads();                                          // lam_s is written; the stages are free
 
     if constexpr (FEW && NW > 1) {
         // join the waves: a common maximum, then the outputs added in wave order
-        float* ml = reinterpret_cast<float*>(smem);           // [NW][32][4]
+        float* ml = reinterpret_cast<float*>(stages);           // [NW][32][4]
         float* acc = ml + NW * 32 * 4;                        // [32][2 DV + 4]
         constexpr int LD = 2 * S::DV + 4;
         if (lh == 0) {
@@ -360,13 +379,13 @@ struct DiffPlan {
 };
 
 // One workgroup per (batch, key head, row tile) unless that leaves CUs idle: then the keys are divided until ~512 workgroups
-// exist (few rows: ~256, one to a CU by their LDS), no split under 256 keys
+// exist (few rows: ~1024, which evens out ragged lengths), no split under 256 keys
 static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv) {
     const int g = H / Hk, rows = Tq * g, hd = diff_head_dim(D, Dv);
     DiffPlan pl{rows <= 32, 1, Tk};
     const int kt = 128;                                       // whole tiles of every variant
     const int64_t units = (int64_t)B * Hk * (pl.few ? 1 : (rows + 127) / 128) * (hd == 128 ? (Dv + 127) / 128 : 1);
-    const int64_t want = (pl.few ? 256 : 512) / (units < 1 ? 1 : units);
+    const int64_t want = (pl.few ? 1024 : 512) / (units < 1 ? 1 : units);
     int64_t splits = want < 1 ? 1 : want;
     const int64_t most = (Tk + 255) / 256;
     if (splits > most) splits = most;
@@ -380,14 +399,11 @@ static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv) {
 
 template <typename T, int HD, bool FEW>
 static int launch_diff(const char* fn, const DiffArgs& a, hipStream_t st) {
-    auto kern = diff_attn_kernel<T, HD, FEW>;
-    static bool attr_set[kMaxDevices] = {};
-    if (int rc = ensure_max_lds(reinterpret_cast<const void*>(kern), attr_set, fn)) return rc;
     const int rows = a.Tq * a.g, per = FEW ? 32 : 128;
     const int vblocks = (a.Dv + DiffShape<T, HD>::DV - 1) / DiffShape<T, HD>::DV;
     const int64_t blocks = (int64_t)a.B * a.Hk * ((rows + per - 1) / per) * a.splits * vblocks;
     NDB_REQUIRE(blocks <= (1 << 24), fn, "too many workgroups for one launch");
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(diff_threads<T, HD, FEW>()), (diff_lds_bytes<T, HD, FEW>()), st, a);
+    hipLaunchKernelGGL((diff_attn_kernel<T, HD, FEW>), dim3((unsigned)blocks), dim3(diff_threads<T, HD, FEW>()), 0, st, a);
     if (a.splits > 1) {
         const int64_t threads = (int64_t)a.B * a.Hk * rows * (a.Dv / 4);
         hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);

@@ -155,7 +155,7 @@ BLOCK_SIGNATURES = {
     'nd_diff_attention': (_T3 * 3 + [_vp] * 4 + [_i64, _f] + [_vp] * 6 + [_i] * 7 + [_f, _i, _i, _vp], _i),
     'nd_diff_attention_workspace_floats': ([_i] * 8, _i64),
     'nd_diff_attention_bwd': (_T3 * 3 + [_vp] * 4 + [_i64, _f] + [_vp] * 4 + _T3 + [_vp] * 8 + [_i] * 7 + [_f, _i, _i, _vp], _i),
-    'nd_diff_attention_bwd_workspace_floats': ([_i] * 5, _i64),
+    'nd_diff_attention_bwd_workspace_floats': ([_i] * 8, _i64),
     'nd_gated_ffn': ([_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp] + [_i] * 5 + [_vp], _i),
     'nd_gated_ffn_workspace_floats': ([_i] * 4, _i64),
     'nd_gated_ffn_bwd': ([_vp, _i64, _vp, _i64] + [_vp] * 11 + [_i] * 5 + [_vp], _i),

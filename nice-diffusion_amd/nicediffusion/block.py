@@ -23,25 +23,24 @@ _DT = {torch.float32: _hip.DT_F32, torch.bfloat16: _hip.DT_BF16}
 
 
 # ------------------------------------------------------------------------------------------------------------ plumbing
-def _check(first, **others):
-    """Device and dtype of a call: every tensor on ``first``'s GPU, in its dtype (float32 / bfloat16).  None is skipped."""
-    name, t = first
+# (a decode step is a few microseconds of kernels: what runs per call below is kept short)
+def _check(name, t, names, others):
+    """Device and dtype of a call: every tensor on the first one's GPU, in its dtype (float32 / bfloat16).  None is skipped."""
     _hip.require_device(t, name)
-    if t.dtype not in _DT:
-        raise TypeError('{} is {}: float32 or bfloat16 expected'.format(name, t.dtype))
-    for n, o in others.items():
-        if o is None:
-            continue
-        if o.device != t.device:
-            raise ValueError('{} lives on {}, {} on {}'.format(n, o.device, name, t.device))
-        if o.dtype != t.dtype:
-            raise TypeError('{} is {}, {} is {}: one dtype per call'.format(n, o.dtype, name, t.dtype))
-    _hip.require_gfx950(t.device.index)
+    dev, dtype = t.device, t.dtype
+    if dtype not in _DT:
+        raise TypeError('{} is {}: float32 or bfloat16 expected'.format(name, dtype))
+    for n, o in zip(names, others):
+        if o is not None and (o.dtype is not dtype or o.device != dev):
+            if o.device != dev:
+                raise ValueError('{} lives on {}, {} on {}'.format(n, o.device, name, dev))
+            raise TypeError('{} is {}, {} is {}: one dtype per call'.format(n, o.dtype, name, dtype))
+    _hip.require_gfx950(dev.index)
 
 
 def _shape(t, name, *want):
-    if t.dim() != len(want) or any(w is not None and s != w for s, w in zip(t.shape, want)):
-        raise ValueError('{} has shape {}, expected {}'.format(name, tuple(t.shape), tuple('?' if w is None else w for w in want)))
+    if t.shape != want:
+        raise ValueError('{} has shape {}, expected {}'.format(name, tuple(t.shape), want))
 
 
 def _rows(t):
@@ -50,19 +49,29 @@ def _rows(t):
 
 
 def _strides(t):
-    """Element strides of the leading dimensions; 0 for a dimension of one element, whose stride says nothing."""
-    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
+    """Element strides of the first three of four dimensions; 0 for a dimension of one element, whose stride says nothing."""
+    (a, b, c, _), (i, j, k, _) = t.stride(), t.shape
+    return (0 if i == 1 else a, 0 if j == 1 else b, 0 if k == 1 else c)
+
+
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def _stream(index):
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def _call(name, device, *args):
     """Launch ``name`` on the current stream of ``device`` (made the current device for the call)."""
     fn = getattr(_hip.load_block(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    _hip.check_block(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        _hip.check_block(rc, name)
 
 
 def _aligned(t):
@@ -78,7 +87,15 @@ def _floats(n, device):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _floats(n, device):
+    return torch.empty(n, dtype=torch.float32, device=device) if n > 0 else None
 
 
 # ------------------------------------------------------------------------------------- query / key norm with rotation
@@ -181,15 +198,20 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
     if q.dim() != 4:
         raise ValueError('q has shape {}, expected [B, T, heads, D]'.format(tuple(q.shape)))
     B, T, Hq, D = q.shape
-    _shape(k, 'k', B, T, None, D)
-    _check(('q', q), k=k, q_weight=q_weight, k_weight=k_weight)
+    if k.dim() != 4:
+        raise ValueError('k has shape {}, expected [B, T, heads, D]'.format(tuple(k.shape)))
+    _shape(k, 'k', B, T, k.shape[2], D)
+    _check('q', q, ('k', 'q_weight', 'k_weight'), (k, q_weight, k_weight))
     if D == 0 or D % 2 or D > 512:
         raise ValueError('head dim must be even and at most 512, got {}'.format(D))
     if Hq == 0 or k.shape[2] == 0:
         raise ValueError('q and k need at least one head')
-    for n, w in (('q_weight', q_weight), ('k_weight', k_weight)):
-        if w is not None:
-            _shape(w, n, D)
+    if q_weight is not None:
+        _shape(q_weight, 'q_weight', D)
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        _shape(k_weight, 'k_weight', D)
+        k_weight = k_weight.contiguous()
     if (cos is None) != (sin is None):
         raise ValueError('cos and sin come together')
     if cos is not None:
@@ -203,7 +225,6 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
         if not 0 < 2 * cos.shape[-1] <= D:
             raise ValueError('tables for {} channels, head dim is {}'.format(2 * cos.shape[-1], D))
     q, k = _rows(q), _rows(k)
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
     if out is not None:
         if _wants_grad(q, k, q_weight, k_weight):
             raise ValueError('out= records no gradient: call under torch.no_grad() or without out')
@@ -212,13 +233,13 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
             _shape(o, n, *t.shape)
             if o.stride(-1) != 1:
                 raise ValueError('{} must have contiguous channels'.format(n))
-        _check(('q', q), **{'out[0]': qo, 'out[1]': ko})
+        _check('q', q, ('out[0]', 'out[1]'), (qo, ko))
         if q.numel():
             _launch_qk(q, k, q_weight, k_weight, cos, sin, eps, interleaved, qo, ko)
         return qo, ko
     if _wants_grad(q, k, q_weight, k_weight):
         return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, eps, interleaved)
-    qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
     if q.numel():
         _launch_qk(q, k, q_weight, k_weight, cos, sin, eps, interleaved, qo, ko)
     return qo, ko
@@ -228,26 +249,29 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
 def _attn_rows(t):
     """``t`` [B, T, heads, channels] as the kernels read it: contiguous channels, every row on a 16-byte boundary (else a copy)."""
     per = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % per for s in _strides(t)) or not 0 <= _strides(t)[1] <= 1 << 22:
+    a, b, c = _strides(t)
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or (a | b | c) % per or b > 1 << 22:
         t = t.contiguous() if not t.is_contiguous() else t.clone()
     return t
 
 
 def _diff_args(q, k, v, lams, lambda_init, lengths):
     per_head = lams[0].dim() == 2
-    return [q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), *(t.data_ptr() for t in lams),
-            lams[0].shape[-1] if per_head else 0, lambda_init, _hip.ptr(lengths)]
+    lq1, lk1, lq2, lk2 = lams
+    return (q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), lq1.data_ptr(), lk1.data_ptr(), lq2.data_ptr(),
+            lk2.data_ptr(), lq1.shape[-1] if per_head else 0, lambda_init, _hip.ptr(lengths))
 
 
 def _diff_sizes(q, k, v):
-    return [q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3] // 2, v.shape[3]]
+    B, Tq, H, D2 = q.shape
+    _, Tk, Hk, Dv = v.shape
+    return (B, Tq, Tk, H, Hk, D2 // 2, Dv)
 
 
 def _launch_diff(q, k, v, lams, lambda_init, scale, lengths, causal, keep):
     B, Tq, Tk, H, Hk, D, Dv = sizes = _diff_sizes(q, k, v)
-    new = dict(dtype=q.dtype, device=q.device)
-    out = torch.empty(B, Tq, H, Dv, **new)
-    o1, o2, lse = (torch.empty(B, Tq, H, Dv, **new), torch.empty(B, Tq, H, Dv, **new), _floats(2 * B * Tq * H, q.device)) if keep else (None,) * 3
+    out = q.new_empty(B, Tq, H, Dv)
+    o1, o2, lse = (torch.empty_like(out), torch.empty_like(out), _floats(2 * B * Tq * H, q.device)) if keep else (None,) * 3
     ws = _floats(_hip.load_block().nd_diff_attention_workspace_floats(*sizes, _DT[q.dtype]), q.device)
     _call('nd_diff_attention', q.device, *_diff_args(q, k, v, lams, lambda_init, lengths), out.data_ptr(), _hip.ptr(o1), _hip.ptr(o2),
           _hip.ptr(lse), _hip.ptr(ws), *sizes, scale, _hip.ATTN_CAUSAL if causal else 0, _DT[q.dtype])
@@ -273,11 +297,15 @@ class _DiffAttention(torch.autograd.Function):
         dout = _attn_rows(dout)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         dl = [torch.empty_like(t) if n else None for t, n in zip(lams, ctx.needs_input_grad[3:7])]
-        ws = _floats(_hip.load_block().nd_diff_attention_bwd_workspace_floats(*sizes[:5]), q.device)
+        ws = _floats(_hip.load_block().nd_diff_attention_bwd_workspace_floats(*sizes, _DT[q.dtype]), q.device)
         _call('nd_diff_attention_bwd', q.device, *_diff_args(q, k, v, lams, ctx.lambda_init, lengths), o1.data_ptr(), o2.data_ptr(),
               lse.data_ptr(), dout.data_ptr(), *_strides(dout), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *(_hip.ptr(t) for t in dl),
               ws.data_ptr(), *sizes, ctx.scale, _hip.ATTN_CAUSAL if ctx.causal else 0, _DT[q.dtype])
         return (dq, dk, dv, *dl, None, None, None, None)
+
+
+_LAMBDAS = ('lambda_q1', 'lambda_k1', 'lambda_q2', 'lambda_k2')
+_DIFF_NAMES = ('k', 'v') + _LAMBDAS
 
 
 def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, lambda_init=0.8, scale=None, key_lengths=None, causal=False):
@@ -294,18 +322,19 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
     a form of their own that divides the keys."""
     if q.dim() != 4 or q.shape[3] % 2:
         raise ValueError('q has shape {}, expected [B, Tq, H, 2 D]'.format(tuple(q.shape)))
-    B, Tq, H, D = q.shape[0], q.shape[1], q.shape[2], q.shape[3] // 2
-    _shape(k, 'k', B, None, None, 2 * D)
-    Tk, Hk = k.shape[1], k.shape[2]
-    _shape(v, 'v', B, Tk, Hk, None)
-    Dv = v.shape[3]
+    B, Tq, H, D = q.shape
+    D //= 2
+    if k.dim() != 4 or v.dim() != 4:
+        raise ValueError('k has shape {}, v {}, expected [B, Tk, Hk, 2 D] and [B, Tk, Hk, Dv]'.format(tuple(k.shape), tuple(v.shape)))
+    _, Tk, Hk, Dv = v.shape
+    _shape(k, 'k', B, Tk, Hk, 2 * D)
+    _shape(v, 'v', B, Tk, Hk, Dv)
     lams = (lambda_q1, lambda_k1, lambda_q2, lambda_k2)
-    names = ('lambda_q1', 'lambda_k1', 'lambda_q2', 'lambda_k2')
-    if tuple(lambda_q1.shape) not in ((D,), (H, D)):
+    if lambda_q1.shape not in ((D,), (H, D)):
         raise ValueError('lambda_q1 has shape {}, expected [{}] or [{}, {}]'.format(tuple(lambda_q1.shape), D, H, D))
-    for n, t in zip(names, lams):
+    for n, t in zip(_LAMBDAS, lams):
         _shape(t, n, *lambda_q1.shape)
-    _check(('q', q), k=k, v=v, **dict(zip(names, lams)))
+    _check('q', q, _DIFF_NAMES, (k, v) + lams)
     if D == 0 or D % 8 or D > 128 or Dv == 0 or Dv % 8 or Dv > 256:
         raise ValueError('D ({}) and Dv ({}) must be positive multiples of 8, at most 128 and 256'.format(D, Dv))
     if H == 0 or Hk == 0 or H % Hk or H // Hk > 64:
@@ -335,7 +364,7 @@ _ACTS = {'silu': _hip.ACT_SILU, 'gelu': _hip.ACT_GELU, 'gelu_tanh': _hip.ACT_GEL
 
 def _matrix(t, cols):
     """``t`` [..., cols] as 16-byte aligned rows [M, cols] (a copy only where it does not lie like that)."""
-    m = t.reshape(-1, cols)
+    m = t if t.dim() == 2 else t.reshape(-1, cols)
     if m.stride(1) != 1 or (m.shape[0] > 1 and not cols <= m.stride(0) <= 1 << 21) or m.stride(0) * m.element_size() % 16 or m.data_ptr() % 16:
         m = m.contiguous() if not m.is_contiguous() else m.clone()
     return m
@@ -348,9 +377,8 @@ def _ld(m):
 def _launch_ffn(x, w_in, b_in, w_out, b_out, res, act, keep):
     M, C = x.shape
     F = w_out.shape[1]
-    new = dict(dtype=x.dtype, device=x.device)
-    y, h = torch.empty(M, C, **new), torch.empty(M, F, **new)
-    au = torch.empty(M, 2 * F, **new) if keep else None
+    y, h = x.new_empty(M, C), x.new_empty(M, F)
+    au = x.new_empty(M, 2 * F) if keep else None
     ws = _floats(_hip.load_block().nd_gated_ffn_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
     _call('nd_gated_ffn', x.device, x.data_ptr(), _ld(x), w_in.data_ptr(), _hip.ptr(b_in), w_out.data_ptr(), _hip.ptr(b_out), _hip.ptr(res),
           0 if res is None else _ld(res), y.data_ptr(), C, h.data_ptr(), _hip.ptr(au), _hip.ptr(ws), M, C, F, act, _DT[x.dtype])
@@ -426,7 +454,7 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, residual=None, act
         _shape(b_out, 'b_out', C)
     if residual is not None:
         _shape(residual, 'residual', *x.shape)
-    _check(('x', x), w_in=w_in, w_out=w_out, b_in=b_in, b_out=b_out, residual=residual)
+    _check('x', x, ('w_in', 'w_out', 'b_in', 'b_out', 'residual'), (w_in, w_out, b_in, b_out, residual))
     if x.numel() // C >= 1 << 31:
         raise ValueError('too many rows')
     act = _ACTS[activation]

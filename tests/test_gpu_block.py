@@ -431,3 +431,20 @@ def test_differential_attention_empty():
         assert o.shape == (B, Tq, 2, 16) and (o == 0).all()
         for g, t in zip(torch.autograd.grad(o.sum(), (q, k, v, *lams)), (q, k, v, *lams)):
             assert g.shape == t.shape and (g == 0).all()
+
+
+def test_differential_attention_rows_that_repeat_in_memory():
+    """Queries, keys and values expanded over tokens (stride 0): rows past the last are not told apart by their address."""
+    for dtype in (BF, F32):
+        B, T, H, D = 2, 45, 2, 32
+        q, k, v = (rnd(B, 1, H, 2 * D, seed=i, dtype=dtype).expand(-1, T, -1, -1) for i in range(3))
+        lams = [rnd(D, seed=4 + i, dtype=dtype, scale=0.2) for i in range(4)]
+        dout = rnd(B, 1, H, 2 * D, seed=9, dtype=dtype).expand(-1, T, -1, -1)
+        ln = torch.tensor([45, 33], dtype=torch.int32, device=DEV)
+        got = []
+        for a, b, c, d in ((q, k, v, dout), [t.contiguous() for t in (q, k, v, dout)]):
+            leaves = [t.detach().requires_grad_() for t in (a, b, c, *lams)]
+            o = block.differential_attention(*leaves, key_lengths=ln)
+            got.append((o, *torch.autograd.grad(o, leaves, d)))
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
