@@ -10,7 +10,11 @@
 // their scales are only known then.  Alternatively the maps could be joined before the product (two thirds of its operations),
 // at the price of a pass over the scores for the statistics: the same matrix operations and twice the exponentials.
 //   prefill    4 waves x 32 rows, tiles of 64 keys (fp32 with D > 64: 32), two stages, loads straight to LDS
-//   few rows   (g Tq <= 32: single tokens) the waves share the rows and divide the keys of a tile; joined in LDS
+//   few rows   (g Tq <= 32: single tokens) a read of the cache: 8 waves (fewer for wide tiles) share the rows, each with a tile of
+//              32 keys of its own, no barrier; the next keys are requested when the scores are made, the next values when the
+//              outputs are, so about 3/4 of 128 KiB a CU is under way.  16 x 16 heads (4 key heads), 64 + 128 channels, ragged
+//              caches up to 8192 (197 MB): 51 us; tiles of 128 keys for the whole workgroup in two stages 62, four 32-key
+//              stages for each of 2 waves 81
 //   wide heads (D > 64) 128 value channels a workgroup, the scores made twice when Dv is above that: both maps' outputs and the
 //              queries of 256 channels do not fit the registers (measured: 290 spilled)
 //   splits     when (batch, key head, row tile) does not fill the chip the keys are divided over workgroups; fp32 partial
@@ -30,31 +34,61 @@ struct DiffShape {
     static constexpr int NS = PH / 2;                        // steps of a score product
     static constexpr int NDT = DV / 32;
     static constexpr int KT_MANY = (ES == 4 && HD == 128) ? 32 : 64;
-    static constexpr int KT_FEW = 128 * (RBK + RBV) <= 32768 ? 128 : (64 * (RBK + RBV) <= 32768 ? 64 : 32);     // two workgroups a CU
+    // few rows: each wave has a tile of 32 keys of its own, up to 128 KiB together
+    static constexpr int TILE_FEW = 32 * (RBK + RBV);
+    static constexpr int NW_FEW = TILE_FEW <= 16384 ? 8 : (TILE_FEW <= 32768 ? 4 : 2);
+    static constexpr int DP_FEW = TILE_FEW >= 16384 ? 2 : 1;  // 32-channel blocks of both maps joined at a time
 };
 
 template <typename T, int HD, bool FEW>
-constexpr int diff_threads() { return FEW ? 2 * DiffShape<T, HD>::KT_FEW : 256; }
+constexpr int diff_threads() { return FEW ? 64 * DiffShape<T, HD>::NW_FEW : 256; }
+
+// four channels dd .. of output row `orow` from both maps' sums and their statistics (maximum, sum of weights, twice)
+template <typename T>
+__device__ __forceinline__ void diff_store(const DiffArgs& p, int64_t orow, int dd, const f32x4 (&o)[2], const f32x4& st, float lam, bool first) {
+    float a[4], c[4], y[4];
+    const float i1 = st[1] != 0.f ? 1.f / st[1] : 0.f, i2 = st[3] != 0.f ? 1.f / st[3] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        a[e] = o[0][e] * i1;
+        c[e] = o[1][e] * i2;
+        y[e] = a[e] - lam * c[e];
+    }
+    store_vec<T, 4>(static_cast<T*>(p.out) + orow * p.Dv + dd, y);
+    if (p.o1) {
+        store_vec<T, 4>(static_cast<T*>(p.o1) + orow * p.Dv + dd, a);
+        store_vec<T, 4>(static_cast<T*>(p.o2) + orow * p.Dv + dd, c);
+    }
+    if (p.lse && first) {
+        p.lse[orow] = st[1] != 0.f ? st[0] + log2f(st[1]) : INFINITY;
+        p.lse[(int64_t)p.B * p.Tq * p.H + orow] = st[3] != 0.f ? st[2] + log2f(st[3]) : INFINITY;
+    }
+}
 
 template <typename T, int HD, bool FEW>
 __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeof(T) >= 256 ? 1 : (HD == 32 && sizeof(T) == 2 && !FEW ? 3 : 2))) diff_attn_kernel(const DiffArgs p) {
     using S = DiffShape<T, HD>;
-    constexpr int KT = FEW ? S::KT_FEW : S::KT_MANY;
-    constexpr int NW = FEW ? KT / 32 : 4;                    // waves
+    constexpr int KT = FEW ? 32 : S::KT_MANY;                // keys of a tile
+    constexpr int NW = FEW ? S::NW_FEW : 4;                  // waves
     constexpr int NJ = 1;                                     // 32-key blocks at a time (2 at D <= 32: 181 registers for 142, no faster)
     constexpr int STAGE = KT * (S::RBK + S::RBV);
-    constexpr int NST = !FEW && HD == 32 && S::ES == 2 ? 3 : 2;                      // tiles in LDS
+    constexpr int NST = HD == 32 && S::ES == 2 ? 3 : 2;       // tiles in LDS (few rows: one a wave)
+    constexpr int LDS = STAGE * (FEW ? NW : NST);
     using TK = Tile<T, S::RBK>;
     using TV = Tile<T, S::RBV>;
-    static_assert(!FEW || NW == 1 || NW * 32 * 16 + 32 * (2 * S::DV + 4) * 4 <= NST * STAGE, "the waves' join fits the stages");
-    __shared__ __attribute__((aligned(16))) char stages[NST * STAGE];
+    static_assert(!FEW || S::DP_FEW * 8192 <= STAGE, "a wave's part of the join fits its tile");
+    __shared__ __attribute__((aligned(16))) char stages[LDS];
     __shared__ float lam_s[DIFF_MAX_GROUP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, lh = lane >> 5;
 
     const int rows = p.Tq * p.g, tiles = (rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
     int bh, id;
-    unit_of(blockIdx.x, gridDim.x, p.B * p.Hk, p.causal, bh, id);
+    if (FEW) {                                                // nothing to share: the (batch, key head)s in turn, so that every XCD
+        id = blockIdx.x / (p.B * p.Hk), bh = blockIdx.x - id * (p.B * p.Hk);      // has long and short sequences
+    } else {
+        unit_of(blockIdx.x, gridDim.x, p.B * p.Hk, p.causal, bh, id);
+    }
     const int vb = HD == 128 ? id / (tiles * p.splits) : 0, dv0 = vb * S::DV, dvn = p.Dv - dv0 < S::DV ? p.Dv - dv0 : S::DV;
     id -= vb * tiles * p.splits;
     const int sp = id / tiles, tile = tiles - 1 - (id - sp * tiles);      // longest rows first
@@ -74,7 +108,7 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
     const int kbeg = sp * p.chunk;
     int kend = kbeg + p.chunk < last ? kbeg + p.chunk : last;
 
-    for (int h = wave; h < p.g; h += NW) {
+    for (int h = wave; h < (p.splits == 1 ? p.g : 0); h += NW) {      // divided keys: the join makes them
         float e1, e2;
         diff_lambda<T>(p, hk * p.g + h, lane, e1, e2);
         if (lane == 0) lam_s[h] = e1 - e2 + p.lam_init;
@@ -101,24 +135,34 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
             for (int e = 0; e < 16; ++e) o[m][d][e] = 0.f;
     float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    TileLoad<T, S::RBK, KT, NW> lk;
-    TileLoad<T, S::RBV, KT, NW> lv;
-    lk.template init<S::RBK / 2>(p.k.st * S::ES, p.D * S::ES, wave, lane);
-    lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, wave, lane);
+    TileLoad<T, S::RBK, KT, FEW ? 1 : NW> lk;
+    TileLoad<T, S::RBV, KT, FEW ? 1 : NW> lv;
+    const int lw = FEW ? 0 : wave;
+    lk.template init<S::RBK / 2>(p.k.st * S::ES, p.D * S::ES, lw, lane);
+    lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, lw, lane);
+    const int tile_step = FEW ? KT * NW : KT, kfirst = FEW ? kbeg + wave * KT : kbeg;      // few rows: the waves take tiles in turn
     const T* kp = static_cast<const T*>(p.k.p) + b * p.k.sb + hk * p.k.sh;
     const T* vp = static_cast<const T*>(p.v.p) + b * p.v.sb + hk * p.v.sh + dv0;
-    auto fetch = [&](int i, char* at) {                       // keys at or past the sequence's end become zero rows
-        const int key = kbeg + i * KT;
+    auto fetch_k = [&](int i, char* at) {                     // keys at or past the sequence's end become zero rows
+        const int key = kfirst + i * tile_step;
         const int64_t n = len - key;
-        lk.load(at, kp + (int64_t)key * p.k.st, ((n - 1) * p.k.st + 2 * p.D) * S::ES, wave);
-        lv.load(at + KT * S::RBK, vp + (int64_t)key * p.v.st, ((n - 1) * p.v.st + dvn) * S::ES, wave);
+        lk.load(at, kp + (int64_t)key * p.k.st, ((n - 1) * p.k.st + 2 * p.D) * S::ES, lw);
+    };
+    auto fetch_v = [&](int i, char* at) {
+        const int key = kfirst + i * tile_step;
+        const int64_t n = len - key;
+        lv.load(at + KT * S::RBK, vp + (int64_t)key * p.v.st, ((n - 1) * p.v.st + dvn) * S::ES, lw);
+    };
+    auto fetch = [&](int i, char* at) {
+        fetch_k(i, at);
+        fetch_v(i, at);
     };
     const int row_base = TK::row_base(lane), col_base = TV::col_base(lane);
-    auto compute = [&](int i, const char* tk) {
-        const int key0 = kbeg + i * KT;
+    auto compute = [&](int i, const char* tk, auto&& scored) {       // scored(): the tile's keys are read
+        const int key0 = kfirst + i * tile_step;
         const char* tv = tk + KT * S::RBK;
 #pragma unroll 1
-        for (int sub = FEW ? wave : 0; sub < (FEW ? wave + 1 : KT / 32); sub += NJ) {
+        for (int sub = 0; sub < KT / 32; sub += NJ) {
             const int kb = key0 + sub * 32;
             if (kb >= kend) break;
             const int rb = in_loop(row_base), cb = in_loop(col_base);
@@ -134,6 +178,7 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
 #pragma unroll
                     for (int c = 0; c < S::NS; ++c) s[m][j] = mma_step<T>(TK::row(k32, rb, 32 * j, m * S::PH + 2 * c), q[m][c], s[m][j]);
                 }
+            scored();
             // scores past what a row sees: only in the tile that holds a row's end
             const bool cut = p.causal ? kb + 32 * NJ > r0 / p.g + len - p.Tq + 1 : kb + 32 * NJ > len;
             if (cut) {
@@ -214,52 +259,98 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
             }
         }
     };
-    ring<NST, decltype(lk)::NI + decltype(lv)::NI>(stages, STAGE, kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0, fetch, compute);
+    const int n = kend > kfirst ? (kend - kfirst + tile_step - 1) / tile_step : 0;
+    if constexpr (FEW) {                                      // the next tile's keys after the scores, its values after the outputs
+        constexpr int NK = decltype(lk)::NI, NV = decltype(lv)::NI;
+        char* mine = stages + wave * STAGE;
+        if (n > 0) fetch(0, mine);
+        for (int i = 0; i < n; ++i) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV) : "memory");      // the tile's keys are there ...
+            compute(i, mine, [&] {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (i + 1 < n) {
+                    fetch_k(i + 1, mine);
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK) : "memory");      // ... and its values
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+            });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (i + 1 < n) fetch_v(i + 1, mine);
+        }
+    } else {
+        ring<NST, decltype(lk)::NI + decltype(lv)::NI>(stages, STAGE, n, fetch, [&](int i, const char* at) { compute(i, at, [] {}); });
+    }
     l[0] = half_sum(l[0]);
     l[1] = half_sum(l[1]);
     __syncthreads();                                          // lam_s is written; the stages are free
 
-    if constexpr (FEW && NW > 1) {
-        // join the waves: a common maximum, then the outputs added in wave order
-        float* ml = reinterpret_cast<float*>(stages);           // [NW][32][4]
-        float* acc = ml + NW * 32 * 4;                        // [32][2 DV + 4]
-        constexpr int LD = 2 * S::DV + 4;
+    if constexpr (FEW) {                                      // join the waves
+        __shared__ float ml[NW][32][4];
         if (lh == 0) {
-            ml[(wave * 32 + l31) * 4 + 0] = mx[0];
-            ml[(wave * 32 + l31) * 4 + 1] = l[0];
-            ml[(wave * 32 + l31) * 4 + 2] = mx[1];
-            ml[(wave * 32 + l31) * 4 + 3] = l[1];
+            ml[wave][l31][0] = mx[0];
+            ml[wave][l31][1] = l[0];
+            ml[wave][l31][2] = mx[1];
+            ml[wave][l31][3] = l[1];
         }
         __syncthreads();
         float f[2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 0; m < 2; ++m) {                         // a common maximum
             float top = -INFINITY, sum = 0.f;
-            for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[(w * 32 + l31) * 4 + 2 * m]);
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][l31][2 * m]);
             const float ref = top == -INFINITY ? 0.f : top;
-            for (int w = 0; w < NW; ++w) sum += ml[(w * 32 + l31) * 4 + 2 * m + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + l31) * 4 + 2 * m] - ref);
+            for (int w = 0; w < NW; ++w) sum += ml[w][l31][2 * m + 1] * __builtin_amdgcn_exp2f(ml[w][l31][2 * m] - ref);
             f[m] = __builtin_amdgcn_exp2f(mx[m] - ref);
             mx[m] = top;
             l[m] = sum;
         }
-        for (int w = 0; w < NW; ++w) {
-            if (wave == w) {
+        __syncthreads();
+        if (wave == 0 && lh == 0) {
+            ml[0][l31][0] = mx[0];
+            ml[0][l31][1] = l[0];
+            ml[0][l31][2] = mx[1];
+            ml[0][l31][3] = l[1];
+        }
+        // then the outputs, DP blocks of 32 channels of both maps at a time: added in wave order, each element by one thread
+        constexpr int DP = S::DP_FEW, PC = DP * 8;            // 16-byte pieces of a row and map
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
+        for (int d0 = 0; d0 < S::NDT; d0 += DP) {
 #pragma unroll
-                    for (int d = 0; d < S::NDT; ++d)
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int g4 = 0; g4 < 4; ++g4) {
-                            f32x4* a = reinterpret_cast<f32x4*>(acc + l31 * LD + m * S::DV + d * 32 + 8 * g4 + 4 * lh);
-                            f32x4 v = {o[m][d][4 * g4] * f[m], o[m][d][4 * g4 + 1] * f[m], o[m][d][4 * g4 + 2] * f[m], o[m][d][4 * g4 + 3] * f[m]};
-                            if (w) v += *a;
-                            *a = v;
-                            if (w == NW - 1) o[m][d][4 * g4] = v[0], o[m][d][4 * g4 + 1] = v[1], o[m][d][4 * g4 + 2] = v[2], o[m][d][4 * g4 + 3] = v[3];
-                        }
+                for (int d = 0; d < DP; ++d)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const f32x16& x = o[m][d0 + d];
+                        const int pc = (m * DP + d) * 8 + 2 * g4 + lh;
+                        *reinterpret_cast<f32x4*>(stages + (wave * 32 + l31) * (2 * PC * 16) + ((pc ^ (l31 & 7)) << 4)) =
+                            f32x4{x[4 * g4] * f[m], x[4 * g4 + 1] * f[m], x[4 * g4 + 2] * f[m], x[4 * g4 + 3] * f[m]};
+                    }
+            __syncthreads();
+            for (int e = threadIdx.x; e < rows * PC; e += NW * 64) {
+                const int row = e / PC, pc = e - row * PC, dd = d0 * 32 + pc * 4;
+                if (dd >= dvn) continue;
+                f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                for (int w = 0; w < NW; ++w)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+                        sum[m] += *reinterpret_cast<const f32x4*>(stages + (w * 32 + row) * (2 * PC * 16) + (((m * PC + pc) ^ (row & 7)) << 4));
+                const f32x4 st = *reinterpret_cast<const f32x4*>(ml[0][row]);
+                const bool first = dd == 0 && vb == 0;
+                if (p.splits > 1) {
+                    float* at = p.part + ((int64_t)sp * p.B * p.Hk * rows + (int64_t)bh * rows + row) * (2 * p.Dv + 4);
+                    *reinterpret_cast<f32x4*>(at + dv0 + dd) = sum[0];
+                    *reinterpret_cast<f32x4*>(at + p.Dv + dv0 + dd) = sum[1];
+                    if (first) *reinterpret_cast<f32x4*>(at + 2 * p.Dv) = st;
+                    continue;
+                }
+                const int tt = row / p.g, h = row - tt * p.g;
+                diff_store<T>(p, ((int64_t)b * p.Tq + tt) * p.H + hk * p.g + h, dv0 + dd, sum, st, lam_s[h], first);
             }
             __syncthreads();
         }
-        if (wave != NW - 1) return;
+        return;
     }
     if (r0 + l31 >= rows) return;
     if (p.splits > 1) {
@@ -277,30 +368,17 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
         if (lh == 0 && vb == 0) *reinterpret_cast<f32x4*>(at + 2 * p.Dv) = f32x4{mx[0], l[0], mx[1], l[1]};
         return;
     }
-    const float i1 = l[0] != 0.f ? 1.f / l[0] : 0.f, i2 = l[1] != 0.f ? 1.f / l[1] : 0.f, lam = lam_s[hg];
+    const f32x4 st = {mx[0], l[0], mx[1], l[1]};
     const int64_t orow = ((int64_t)b * p.Tq + t) * p.H + head;
-    if (p.lse && lh == 0 && vb == 0) {
-        p.lse[orow] = l[0] != 0.f ? mx[0] + log2f(l[0]) : INFINITY;
-        p.lse[(int64_t)p.B * p.Tq * p.H + orow] = l[1] != 0.f ? mx[1] + log2f(l[1]) : INFINITY;
-    }
 #pragma unroll
     for (int d = 0; d < S::NDT; ++d)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
             const int dd = d * 32 + 8 * g4 + 4 * lh;
-            if (dd >= dvn) continue;
-            float a[4], c[4], y[4];
+            f32x4 sum[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[e] = o[0][d][4 * g4 + e] * i1;
-                c[e] = o[1][d][4 * g4 + e] * i2;
-                y[e] = a[e] - lam * c[e];
-            }
-            store_vec<T, 4>(static_cast<T*>(p.out) + orow * p.Dv + dv0 + dd, y);
-            if (p.o1) {
-                store_vec<T, 4>(static_cast<T*>(p.o1) + orow * p.Dv + dv0 + dd, a);
-                store_vec<T, 4>(static_cast<T*>(p.o2) + orow * p.Dv + dv0 + dd, c);
-            }
+            for (int m = 0; m < 2; ++m) sum[m] = f32x4{o[m][d][4 * g4], o[m][d][4 * g4 + 1], o[m][d][4 * g4 + 2], o[m][d][4 * g4 + 3]};
+            if (dd < dvn) diff_store<T>(p, orow, dv0 + dd, sum, st, lam_s[hg], dd == 0 && vb == 0);
         }
 }
 
@@ -346,25 +424,8 @@ __global__ void __launch_bounds__(256) diff_join_kernel(const DiffArgs p) {
             e2 = fmaf(x[2][e], x[3][e], e2);
         }
     }
-    const float lam = expf(e1) - expf(e2) + p.lam_init;
-    const int64_t orow = ((int64_t)b * p.Tq + t) * p.H + head;
-    float a[4], c[4], y[4];
-    const float i1 = l[0] != 0.f ? 1.f / l[0] : 0.f, i2 = l[1] != 0.f ? 1.f / l[1] : 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        a[e] = o[0][e] * i1;
-        c[e] = o[1][e] * i2;
-        y[e] = a[e] - lam * c[e];
-    }
-    store_vec<T, 4>(static_cast<T*>(p.out) + orow * p.Dv + dd, y);
-    if (p.o1) {
-        store_vec<T, 4>(static_cast<T*>(p.o1) + orow * p.Dv + dd, a);
-        store_vec<T, 4>(static_cast<T*>(p.o2) + orow * p.Dv + dd, c);
-    }
-    if (p.lse && dd == 0) {
-        p.lse[orow] = l[0] != 0.f ? top[0] + log2f(l[0]) : INFINITY;
-        p.lse[(int64_t)p.B * p.Tq * p.H + orow] = l[1] != 0.f ? top[1] + log2f(l[1]) : INFINITY;
-    }
+    const f32x4 st = {top[0], l[0], top[1], l[1]};
+    diff_store<T>(p, ((int64_t)b * p.Tq + t) * p.H + head, dd, o, st, expf(e1) - expf(e2) + p.lam_init, dd == 0);
 }
 
 // padded head dim of the kernels: the smallest of 32 / 64 / 128 that holds D and half of Dv
@@ -379,13 +440,14 @@ struct DiffPlan {
 };
 
 // One workgroup per (batch, key head, row tile) unless that leaves CUs idle: then the keys are divided until ~512 workgroups
-// exist (few rows: ~1024, which evens out ragged lengths), no split under 256 keys
+// exist, no split under 256 keys.  Few rows: ~256, one for each CU (the case above: 51 us; 512 even out ragged lengths, but a
+// second start and join cost more: 58 us, 1024: 74)
 static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv) {
     const int g = H / Hk, rows = Tq * g, hd = diff_head_dim(D, Dv);
     DiffPlan pl{rows <= 32, 1, Tk};
     const int kt = 128;                                       // whole tiles of every variant
     const int64_t units = (int64_t)B * Hk * (pl.few ? 1 : (rows + 127) / 128) * (hd == 128 ? (Dv + 127) / 128 : 1);
-    const int64_t want = (pl.few ? 1024 : 512) / (units < 1 ? 1 : units);
+    const int64_t want = (pl.few ? 256 : 512) / (units < 1 ? 1 : units);
     int64_t splits = want < 1 ? 1 : want;
     const int64_t most = (Tk + 255) / 256;
     if (splits > most) splits = most;
