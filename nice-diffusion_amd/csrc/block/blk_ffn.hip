@@ -250,6 +250,107 @@ __global__ void __launch_bounds__(1024) colsum_join_kernel(const float* part, in
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------ few rows
+// Up to 32 rows: a read of the weights.  A workgroup makes 16 columns (gated: the gate and the up columns of 16 f) of
+// [M, N] = x w^T with 16 x 16 products, the weights' rows as their first operand; its waves take 128-byte pieces of the rows in
+// turn, straight to registers, UNITS pieces requested at a time (bf16 4, fp32 2: 23 us for 24 at 1 x 1024 x 4096), and are summed
+// in wave order.  Both operands take the channels of a piece in the same order, 16 bytes a lane.  Where columns are few (no more
+// than one workgroup a CU) 8 columns: half of the operand stays empty, but twice the CUs read: 12.8 us for 13.9.
+// The block at C 1024, F 4096, bf16 (25 MB, 4.9 us as a copy): 1 row 12.8 us, the tile kernels 28; 32 rows 21 for 30; 33: tiles.
+// What is left are two launches that each start, read for 2 to 3 us and drain.
+constexpr int FEW_ROWS = 32, FEW_NARROW = 2048;
+
+template <typename T, int NW, int MT, int COLS, class Epi>
+__global__ void __launch_bounds__(NW * 64) few_rows_kernel(const T* x, int64_t ldx, const T* w, int M, int N, int K, const Epi epi) {
+    constexpr int G = Epi::GATED ? 2 : 1, PIECE = 128 / (int)sizeof(T), LANE = 16 / (int)sizeof(T), UNITS = sizeof(T) == 2 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) float red[NW][G][16 * MT][20];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, l4 = lane >> 4, n0 = blockIdx.x * COLS;
+    const T* rows[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) rows[g] = w + ((int64_t)g * N + n0 + l15) * K + l4 * LANE;
+    const bool in_n = l15 < COLS && n0 + l15 < N;
+    const int pieces = (K + PIECE - 1) / PIECE;
+    f32x4 acc[MT][G];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int g = 0; g < G; ++g) acc[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int p0 = wave; p0 < pieces; p0 += NW * UNITS) {
+        u32x4 a[UNITS][2][G], b[UNITS][2][MT];
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = (p0 + i * NW) * PIECE + h * (PIECE / 2);
+                const bool in_k = k + l4 * LANE < K;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    a[i][h][g] = u32x4{0u, 0u, 0u, 0u};
+                    if (in_k && in_n) a[i][h][g] = *reinterpret_cast<const u32x4*>(rows[g] + k);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    b[i][h][t] = u32x4{0u, 0u, 0u, 0u};
+                    if (in_k && 16 * t + l15 < M) b[i][h][t] = *reinterpret_cast<const u32x4*>(x + (16 * t + l15) * ldx + l4 * LANE + k);
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        if constexpr (sizeof(T) == 2) {
+                            union { u32x4 u; bf16x8 v; } p, q;
+                            p.u = a[i][h][g], q.u = b[i][h][t];
+                            acc[t][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p.v, q.v, acc[t][g], 0, 0, 0);
+                        } else {
+                            union { u32x4 u; float f[4]; } p, q;
+                            p.u = a[i][h][g], q.u = b[i][h][t];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[t][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(p.f[e], q.f[e], acc[t][g], 0, 0, 0);
+                        }
+                    }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int g = 0; g < G; ++g) *reinterpret_cast<f32x4*>(&red[wave][g][16 * t + l15][l4 * 4]) = acc[t][g];
+    const int m = threadIdx.x / (COLS / 8), c8 = (threadIdx.x % (COLS / 8)) * 8, n = n0 + c8;
+    const bool mine = m < M && n < N;                         // 8 columns of a row (N is a multiple of 8)
+    typename Epi::Cols cols{};
+    typename Epi::Row row{};
+    if (mine) {
+        cols = epi.columns(n);
+        row = epi.row(m, n);
+    }
+    __syncthreads();
+    if (!mine) return;
+    float v[G][8];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            f32x4 t = *reinterpret_cast<const f32x4*>(&red[0][g][m][c8 + e]);
+#pragma unroll
+            for (int u = 1; u < NW; ++u) t += *reinterpret_cast<const f32x4*>(&red[u][g][m][c8 + e]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[g][e + j] = t[j];
+        }
+    epi.store(m, n, 0, v[0], v[G - 1], cols, row);
+}
+
+template <typename T, int NW, class Epi>
+static int run_few(const char* fn, const T* x, int64_t ldx, const T* w, int M, int N, int K, const Epi& epi, hipStream_t st) {
+    const int cols = N <= FEW_NARROW ? 8 : 16;
+    auto kern = M <= 16 ? (cols == 8 ? few_rows_kernel<T, NW, 1, 8, Epi> : few_rows_kernel<T, NW, 1, 16, Epi>)
+                        : (cols == 8 ? few_rows_kernel<T, NW, 2, 8, Epi> : few_rows_kernel<T, NW, 2, 16, Epi>);
+    hipLaunchKernelGGL(kern, dim3((N + cols - 1) / cols), dim3(NW * 64), 0, st, x, ldx, w, M, N, K, epi);
+    return check_launch(fn);
+}
+
 // ------------------------------------------------------------------------------------------------------ launch choices
 struct Plan {
     int big;              // 256 x 256 tiles (else 128 x 128)
@@ -351,12 +452,16 @@ struct Ffn {
 
 template <typename T, int ACT>
 static int ffn_forward(const char* fn, const Ffn<T>& a, hipStream_t st) {
+    const EpiGate<T, ACT> gate{a.b_in, a.h, a.au, a.F};
+    const EpiOut<T> down{a.b_out, a.res, a.y, a.ldr, a.ldy};
+    if (a.M <= FEW_ROWS) {
+        if (int rc = run_few<T, 8>(fn, a.x, a.ldx, a.w_in, a.M, a.F, a.C, gate, st)) return rc;
+        return run_few<T, 16>(fn, a.h, a.F, a.w_out, a.M, a.C, a.F, down, st);
+    }
     const Plan pl = plan_gemm(a.M, a.F, a.C, sizeof(T), true, false);
-    if (int rc = run_gemm<T, true, true>(fn, GemmSide<T>{a.x, a.ldx, a.M}, GemmSide<T>{a.w_in, a.C, 2 * a.F}, a.C, pl, a.F,
-                                         EpiGate<T, ACT>{a.b_in, a.h, a.au, a.F}, st))
+    if (int rc = run_gemm<T, true, true>(fn, GemmSide<T>{a.x, a.ldx, a.M}, GemmSide<T>{a.w_in, a.C, 2 * a.F}, a.C, pl, a.F, gate, st))
         return rc;
-    return run_gemm_out<T, true, true>(fn, GemmSide<T>{a.h, a.F, a.M}, GemmSide<T>{a.w_out, a.F, a.C}, a.F, a.ws,
-                                       EpiOut<T>{a.b_out, a.res, a.y, a.ldr, a.ldy}, st);
+    return run_gemm_out<T, true, true>(fn, GemmSide<T>{a.h, a.F, a.M}, GemmSide<T>{a.w_out, a.F, a.C}, a.F, a.ws, down, st);
 }
 
 template <typename T>
@@ -413,7 +518,7 @@ using namespace ndb;
 
 extern "C" int64_t nd_gated_ffn_workspace_floats(int M, int C, int F, int dtype) {
     if (M <= 0 || C <= 0 || F <= 0) return -1;
-    return split_floats(M, C, F, dtype == ND_DT_BF16 ? 2 : 4);
+    return M <= FEW_ROWS ? 0 : split_floats(M, C, F, dtype == ND_DT_BF16 ? 2 : 4);
 }
 
 extern "C" int nd_gated_ffn(const void* x, int64_t ldx, const void* w_in, const void* b_in, const void* w_out, const void* b_out,
