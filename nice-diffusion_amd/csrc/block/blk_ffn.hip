@@ -504,7 +504,7 @@ static int ffn_backward(const char* fn, const FfnBwd<T>& a, hipStream_t st) {
 static int ffn_check(const char* fn, int M, int C, int F, int act, int dtype) {
     NDB_REQUIRE(M > 0 && C > 0 && F > 0, fn, "sizes must be positive");
     NDB_REQUIRE(C % 8 == 0 && F % 8 == 0, fn, "channels and hidden channels must be multiples of 8");
-    NDB_REQUIRE((int64_t)C * F <= (1LL << 28), fn, "weights of more than 2^28 elements");
+    NDB_REQUIRE((int64_t)C * F <= (1LL << 28) && C <= (1 << 20) && F <= (1 << 20), fn, "weights of more than 2^28 elements, or more than 2^20 channels");
     NDB_REQUIRE(act >= ND_ACT_SILU && act <= ND_ACT_GELU_TANH, fn, "unknown activation");
     NDB_REQUIRE(dtype == ND_DT_F32 || dtype == ND_DT_BF16, fn, "dtype must be ND_DT_F32 or ND_DT_BF16");
     return ND_OK;

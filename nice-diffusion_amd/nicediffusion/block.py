@@ -38,6 +38,19 @@ def _check(name, t, names, others):
     _hip.require_gfx950(dev.index)
 
 
+class _Nothing(torch.autograd.Function):
+    """A result without work: zeros of ``shape`` that every input gets a zero gradient from."""
+    @staticmethod
+    def forward(ctx, shape, *tensors):
+        ctx.tensors = [(t.shape, t.dtype, t.device) for t in tensors]
+        return tensors[0].new_zeros(shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _):
+        return (None, *(torch.zeros(s, dtype=d, device=v) for s, d, v in ctx.tensors))
+
+
 def _shape(t, name, *want):
     if t.shape != want:
         raise ValueError('{} has shape {}, expected {}'.format(name, tuple(t.shape), want))
@@ -94,10 +107,6 @@ def _wants_grad(*tensors):
     return False
 
 
-def _floats(n, device):
-    return torch.empty(n, dtype=torch.float32, device=device) if n > 0 else None
-
-
 # ------------------------------------------------------------------------------------- query / key norm with rotation
 def grid_positions(height, width, device=None):
     """[height * width, 2] (row, column) of the tokens of an NHWC map, in token order."""
@@ -109,13 +118,15 @@ def rotary_table(positions, channels, theta=10000.0):
     """cos and sin tables for ``qk_norm_rope``: fp32 [..., channels / 2] each.
 
     ``positions`` [...] (one axis) or [..., axes]: the pairs are divided evenly among the axes; pair i of an axis' n turns by
-    ``position * theta ** (-i / n)``.  Angles are formed in float64: far positions keep their phase.  A 2-D tensor is read as
-    [..., axes] when its last dimension is at most 3; give a [B, T] batch of one-axis positions as [B, T, 1]."""
+    ``position * theta ** (-i / n)``.  Angles are formed in float64: far positions keep their phase.  Tensors of two and
+    more dimensions end in the axes (at most 3): a [B, T] batch of one-axis positions is given as [B, T, 1]."""
     if channels <= 0 or channels % 2:
         raise ValueError('channels must be positive and even, got {}'.format(channels))
     p = positions.double()
-    if p.dim() == 1 or p.shape[-1] > 3:
-        p = p[..., None]
+    if p.dim() == 1:
+        p = p[:, None]
+    if p.dim() == 0 or not 1 <= p.shape[-1] <= 3:
+        raise ValueError('positions have shape {}, expected [T] or [..., axes] with at most 3 axes'.format(tuple(positions.shape)))
     axes, pairs = p.shape[-1], channels // 2
     if pairs % axes:
         raise ValueError('{} pairs do not divide among {} axes'.format(pairs, axes))
@@ -201,7 +212,6 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
     if k.dim() != 4:
         raise ValueError('k has shape {}, expected [B, T, heads, D]'.format(tuple(k.shape)))
     _shape(k, 'k', B, T, k.shape[2], D)
-    _check('q', q, ('k', 'q_weight', 'k_weight'), (k, q_weight, k_weight))
     if D == 0 or D % 2 or D > 512:
         raise ValueError('head dim must be even and at most 512, got {}'.format(D))
     if Hq == 0 or k.shape[2] == 0:
@@ -224,6 +234,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
             cos, sin = cos.contiguous(), sin.contiguous()
         if not 0 < 2 * cos.shape[-1] <= D:
             raise ValueError('tables for {} channels, head dim is {}'.format(2 * cos.shape[-1], D))
+    _check('q', q, ('k', 'q_weight', 'k_weight'), (k, q_weight, k_weight))
     q, k = _rows(q), _rows(k)
     if out is not None:
         if _wants_grad(q, k, q_weight, k_weight):
@@ -231,9 +242,13 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
         qo, ko = out
         for n, o, t in (('out[0]', qo, q), ('out[1]', ko, k)):
             _shape(o, n, *t.shape)
-            if o.stride(-1) != 1:
-                raise ValueError('{} must have contiguous channels'.format(n))
+            if o.stride(-1) != 1 or 0 in [a for a, z in zip(o.stride(), o.shape) if z > 1]:
+                raise ValueError('{} must have contiguous channels and no rows that repeat'.format(n))
+            if o.data_ptr() == t.data_ptr() and _strides(o) != _strides(t):
+                raise ValueError('{} begins where its input does but lies differently'.format(n))
         _check('q', q, ('out[0]', 'out[1]'), (qo, ko))
+        if q.numel() and qo.data_ptr() in (k.data_ptr(), ko.data_ptr()) or k.numel() and ko.data_ptr() == q.data_ptr():
+            raise ValueError('out must be the inputs themselves, in their order, or other memory')
         if q.numel():
             _launch_qk(q, k, q_weight, k_weight, cos, sin, eps, interleaved, qo, ko)
         return qo, ko
@@ -334,7 +349,6 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
         raise ValueError('lambda_q1 has shape {}, expected [{}] or [{}, {}]'.format(tuple(lambda_q1.shape), D, H, D))
     for n, t in zip(_LAMBDAS, lams):
         _shape(t, n, *lambda_q1.shape)
-    _check('q', q, _DIFF_NAMES, (k, v) + lams)
     if D == 0 or D % 8 or D > 128 or Dv == 0 or Dv % 8 or Dv > 256:
         raise ValueError('D ({}) and Dv ({}) must be positive multiples of 8, at most 128 and 256'.format(D, Dv))
     if H == 0 or Hk == 0 or H % Hk or H // Hk > 64:
@@ -348,10 +362,11 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
             raise TypeError('key_lengths is {}: int32 or int64 expected'.format(key_lengths.dtype))
         if key_lengths.device != q.device:
             raise ValueError('key_lengths lives on {}, q on {}'.format(key_lengths.device, q.device))
+    _check('q', q, _DIFF_NAMES, (k, v) + lams)
+    if key_lengths is not None:
         key_lengths = (key_lengths.clamp(0, Tk) if key_lengths.dtype == torch.int64 else key_lengths).to(torch.int32).contiguous()
     if B == 0 or Tq == 0 or Tk == 0:        # nothing to see: zeros that every input's gradient (zero) flows through
-        out = torch.zeros(B, Tq, H, Dv, dtype=q.dtype, device=q.device)
-        return out + 0 * sum(t.sum() for t in (q, k, v) + lams) if _wants_grad(q, k, v, *lams) else out
+        return _Nothing.apply((B, Tq, H, Dv), q, k, v, *lams)
     if _wants_grad(q, k, v, *lams):
         return _DiffAttention.apply(q, k, v, *lams, float(lambda_init), scale, key_lengths, bool(causal))
     return _launch_diff(_attn_rows(q), _attn_rows(k), _attn_rows(v), [_aligned(t) for t in lams], float(lambda_init), scale, key_lengths,
@@ -446,17 +461,17 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, residual=None, act
     _shape(w_out, 'w_out', C, F)
     if C == 0 or F == 0 or C % 8 or F % 8:
         raise ValueError('channels ({}) and hidden channels ({}) must be positive multiples of 8'.format(C, F))
-    if C * F > 1 << 28:
-        raise ValueError('weights of more than 2^28 elements')
+    if C * F > 1 << 28 or C > 1 << 20 or F > 1 << 20:
+        raise ValueError('weights of more than 2^28 elements, or more than 2^20 channels')
     if b_in is not None:
         _shape(b_in, 'b_in', 2 * F)
     if b_out is not None:
         _shape(b_out, 'b_out', C)
     if residual is not None:
         _shape(residual, 'residual', *x.shape)
-    _check('x', x, ('w_in', 'w_out', 'b_in', 'b_out', 'residual'), (w_in, w_out, b_in, b_out, residual))
     if x.numel() // C >= 1 << 31:
         raise ValueError('too many rows')
+    _check('x', x, ('w_in', 'w_out', 'b_in', 'b_out', 'residual'), (w_in, w_out, b_in, b_out, residual))
     act = _ACTS[activation]
     if _wants_grad(x, w_in, b_in, w_out, b_out, residual):
         return _GatedFfn.apply(x, w_in, b_in, w_out, b_out, residual, act)
