@@ -2,14 +2,15 @@
 // either order ("K-major": rows of consecutive k; otherwise rows of consecutive m / n), the epilogue a functor.
 //
 // A workgroup of 4 waves (2 x 2) makes a tile of 64 TI x 64 TI outputs, a wave 32 TI x 32 TI: TI = 4 (256 x 256, one
-// workgroup a CU) or 2 (128 x 128, two).  Both operands go straight from memory to LDS (buffer loads with the LDS
+// workgroup a CU), 2 (128 x 128, two) or 1 (64 x 64, four: small products, and fp32, whose matrix rate leaves LDS time to spare).  Both operands go straight from memory to LDS (buffer loads with the LDS
 // destination, 16 bytes a lane) in two stages of 128 bytes of k; a wave reads one 16-byte piece a lane and k-step for each
 // of its 32-row fragments, 2 TI of them for TI^2 matrix instructions.  The weights are the first operand of the matrix
 // instruction, so a lane ends with 4 consecutive n of one m.
 //
 //   LDS images   K-major: [row][8 pieces of 16 bytes], piece c of row r at c ^ (r >> 1 & 7): 16 rows read at one piece cover
 //                all 64 banks.  Otherwise [k][row], bf16 read back transposed (ds_read_b64_tr_b16: 4 k of 16 rows), piece c
-//                of k at c ^ (k & 3) << 2; fp32 read one float a lane, piece c at c ^ (k >> 2 & 1) << 3: conflict-free too.
+//                of k at c ^ (k & 3) << 2 (TI = 1, rows of half the banks: c ^ (k >> 1 & 1) << 2); fp32 read one float a lane, piece c at
+//                c ^ (k >> 2 & 1) << 3: conflict-free too.
 //   bf16 k-step  16 k: lane half lh holds k = 8 lh + 0 .. 7 of its row (v_mfma_f32_32x32x16_bf16).
 //   fp32 k-step  8 k:  lane half lh holds k = 4 lh + 0 .. 3; four v_mfma_f32_32x32x2_f32, each taking one k of either half.
 //   Loop         the fragments of a k-step are requested one step ahead; behind the last request of a stage one barrier
@@ -121,7 +122,7 @@ struct GemmOperand {
         }
     }
 
-    static __device__ __forceinline__ int swz(int k) { return ES == 2 ? (k & 3) << 2 : ((k >> 2) & 1) << 3; }
+    static __device__ __forceinline__ int swz(int k) { return ES == 4 ? ((k >> 2) & 1) << 3 : (TI == 1 ? ((k >> 1) & 1) << 2 : (k & 3) << 2); }
 
     __device__ __forceinline__ void one(char* stage, int wave, int i, unsigned n, unsigned o) const {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, (int)n, 0x00020000);
@@ -151,7 +152,7 @@ struct GemmOperand {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int k = 16 * s + 8 * lh + 4 * h + (i >> 2);
-                const char* a = stage + k * ROWB + (((m >> 3) ^ ((i >> 2) << 2)) << 4) + (m & 4) * 2;
+                const char* a = stage + k * ROWB + (((m >> 3) ^ swz(i >> 2)) << 4) + (m & 4) * 2;
                 const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
                 union { s16x4 h4; unsigned u[2]; } c;
                 c.h4 = r;
@@ -189,10 +190,11 @@ __device__ __forceinline__ void gemm_step(const char* src, char* dst, const X& x
             const int i = a * TI + b;
             if (i < TI) fw[c ^ 1][i] = w.frag(src + SZ, lane, i, s);
             else if (i < 2 * TI) fx[c ^ 1][i - TI] = x.frag(src, lane, i - TI, s);
+            if (TI == 1) fx[c ^ 1][0] = x.frag(src, lane, 0, s);
             if (REQ) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    if ((TI == 4 ? j : j / 2) != i) continue;          // PER = TI^2 of them at TI = 4, 2 TI^2 at 2
+                    if (j * TI * TI / PER != i) continue;              // spread over the matrix instructions
                     if (j < X::NL) x.one(dst, wave, j, x.num, x.off[j % X::NL]);
                     else w.one(dst + SZ, wave, j - X::NL, w.num, w.off[(j - X::NL) % W::NL]);
                 }
@@ -235,7 +237,7 @@ __device__ __forceinline__ int gemm_loop(char* __restrict__ sa, char* __restrict
 #undef NDB_SB
 
 template <typename T, int TI, bool XK, bool WK, class Epi>
-__global__ void __launch_bounds__(GEMM_THREADS, TI == 4 ? 1 : 2) gemm_kernel(const GemmArgs<T> p, const Epi epi) {
+__global__ void __launch_bounds__(GEMM_THREADS, 4 / TI) gemm_kernel(const GemmArgs<T> p, const Epi epi) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     using X = GemmOperand<T, TI, XK>;
     using W = GemmOperand<T, TI, WK>;
