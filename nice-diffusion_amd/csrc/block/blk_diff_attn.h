@@ -156,9 +156,10 @@ struct Probs<float> {
     }
 };
 
-// acc[n][d][column] += sum over the 32 rows r0 .. of tile[row][col + 32 n + d] * p[row][column], for N blocks of columns
+// acc[n][d][column] += sum over the 32 rows r0 .. of tile[row][col + 32 n + d] * p[row][column], for N blocks of columns, of which
+// the first `real` columns count (fp32 leaves out blocks past them, D > 64 excepted: see no_step)
 template <typename T, int RB, int N>
-__device__ __forceinline__ void mma_cols(const char* t, int base, int r0, int col, const Probs<T>& p, f32x16 (&acc)[N]) {
+__device__ __forceinline__ void mma_cols(const char* t, int base, int r0, int col, int real, const Probs<T>& p, f32x16 (&acc)[N]) {
     if constexpr (sizeof(T) == 2) {
         static_assert(N % 2 == 0, "blocks in pairs");
 #pragma unroll
@@ -175,17 +176,27 @@ __device__ __forceinline__ void mma_cols(const char* t, int base, int r0, int co
                 }
         }
     } else {
+        if constexpr (RB < 1024) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+            for (int n = 0; n < N; ++n) {
+                if (n && 32 * n >= real) break;
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(Tile<T, RB>::one(t, base, r0, e, col + 32 * n), p.f[e], acc[n], 0, 0, 0);
+                for (int e = 0; e < 16; ++e)
+                    acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(Tile<T, RB>::one(t, base, r0, e, col + 32 * n), p.f[e], acc[n], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(Tile<T, RB>::one(t, base, r0, e, col + 32 * n), p.f[e], acc[n], 0, 0, 0);
+        }
     }
 }
 
 // both maps' products with the halves of one tile: acc[m][d][column] += sum over rows of tile[row][m HD + 32 d ..] * p[m][row][column]
 template <typename T, int RB, int HD>
-__device__ __forceinline__ void mma_halves(const char* t, int base, const Probs<T>& p0, const Probs<T>& p1, f32x16 (&acc)[2][HD / 32]) {
+__device__ __forceinline__ void mma_halves(const char* t, int base, int real, const Probs<T>& p0, const Probs<T>& p1, f32x16 (&acc)[2][HD / 32]) {
     if constexpr (sizeof(T) == 2 && HD == 32) {              // one block of each half: a pair
         u32x4 f[2][2];
         Tile<T, RB>::cols2(t, base, 0, 0, f);
@@ -197,10 +208,15 @@ __device__ __forceinline__ void mma_halves(const char* t, int base, const Probs<
             acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b.h, p1.f[s], acc[1][0], 0, 0, 0);
         }
     } else {
-        mma_cols<T, RB>(t, base, 0, 0, p0, acc[0]);
-        mma_cols<T, RB>(t, base, 0, HD, p1, acc[1]);
+        mma_cols<T, RB>(t, base, 0, 0, real, p0, acc[0]);
+        mma_cols<T, RB>(t, base, 0, HD, real, p1, acc[1]);
     }
 }
+
+// fp32: step c of a product over `real` channels (8 a step) has none left.  A branch costs little beside a step's 256 cycles
+// (D = 48, Dv = 96: 123 us for 140), but not where the registers are full already (D > 64: 255 us for 222 at 128).
+template <typename T, int HD>
+__device__ __forceinline__ bool no_step(int c, int real) { return sizeof(T) == 4 && HD < 128 && c && 8 * c >= real; }
 
 struct DiffTensor {       // [batch, token, head, channel], channels contiguous
     const void* p;

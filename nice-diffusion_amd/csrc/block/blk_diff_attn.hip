@@ -176,7 +176,8 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[m][j][e] = 0.f;
 #pragma unroll
-                    for (int c = 0; c < S::NS; ++c) s[m][j] = mma_step<T>(TK::row(k32, rb, 32 * j, m * S::PH + 2 * c), q[m][c], s[m][j]);
+                    for (int c = 0; c < S::NS; ++c)
+                        if (!no_step<T, HD>(c, p.D)) s[m][j] = mma_step<T>(TK::row(k32, rb, 32 * j, m * S::PH + 2 * c), q[m][c], s[m][j]);
                 }
             scored();
             // scores past what a row sees: only in the tile that holds a row's end
@@ -248,13 +249,15 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
                     }
                 } else {
 #pragma unroll
-                    for (int d = 0; d < S::NDT; ++d)
+                    for (int d = 0; d < S::NDT; ++d) {
+                        if (HD < 128 && d && 32 * d >= dvn) break;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const float a = TV::one(v32, cb, 32 * j, e, d * 32);
                             o[0][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[0][j].f[e], o[0][d], 0, 0, 0);
                             o[1][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pr[1][j].f[e], o[1][d], 0, 0, 0);
                         }
+                    }
                 }
             }
         }
@@ -439,23 +442,51 @@ struct DiffPlan {
     int splits, chunk;
 };
 
-// One workgroup per (batch, key head, row tile) unless that leaves CUs idle: then the keys are divided until ~512 workgroups
-// exist, no split under 256 keys.  Few rows: ~256, one for each CU (the case above: 51 us; 512 even out ragged lengths, but a
-// second start and join cost more: 58 us, 1024: 74)
-static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv) {
+// Into how many parts `length` (keys, rows) is divided: the fewest rounds of workgroups x their time, plus the join.  `units`
+// workgroups without a division, `slots` of them on the chip at a time, `per` cycles of a CU per unit of length and workgroup,
+// `bytes` of fp32 partials per part, written and read at ~5 TB/s (2.3 KiB a cycle); shares are multiples of `grain`.  Causal ones
+// are of all lengths and start with the longest, so rounds say little: none from 256 workgroups on (8 x 2048^2 x 8 heads with
+// gradients: 540 us, 710 divided), else about 512 (1 x 4096^2, 4 heads on one: 190 us, 246 by the rounds).
+int diff_parts(int64_t units, int slots, int64_t length, int64_t grain, double per, double bytes, int causal, int64_t& share) {
+    double best_t = 1e300;
+    int best = 1;
+    share = length;
+    if (causal) {
+        int64_t n = units < 256 ? 512 / units : 1, most = (int64_t)((double)length * per / 24000.0) + 1;      // no share under 24000 cycles
+        n = n < 1 ? 1 : (n < 16 ? n : 16);
+        n = n < most ? n : most;
+        share = ((length + n - 1) / n + grain - 1) / grain * grain;
+        return (int)((length + share - 1) / share);
+    }
+    for (int want = 1; want <= 64; ++want) {
+        const int64_t chunk = ((length + want - 1) / want + grain - 1) / grain * grain, parts = (length + chunk - 1) / chunk;
+        if (parts != want) continue;
+        const int64_t rounds = (units * parts + slots - 1) / slots, active = units * parts < slots ? (units * parts + 255) / 256 : slots / 256;
+        double t = (double)rounds * ((double)chunk * per * active + 6000.0);
+        if (parts > 1) t += 9000.0 + 300.0 * (double)parts + 2.0 * (double)parts * bytes / 2340.0;
+        if (t < best_t) best_t = t, best = (int)parts, share = chunk;
+    }
+    return best;
+}
+
+// Few rows: ~256 workgroups, one for each CU, no split under 256 keys (the case above: 51 us; 512 even out ragged lengths, but a
+// second start and join cost more: 58 us, 1024: 74).  Many: a workgroup's 32 keys take its CU ~30 HD cycles, fp32 ~190 HD.
+static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int es, int causal) {
     const int g = H / Hk, rows = Tq * g, hd = diff_head_dim(D, Dv);
     DiffPlan pl{rows <= 32, 1, Tk};
-    const int kt = 128;                                       // whole tiles of every variant
     const int64_t units = (int64_t)B * Hk * (pl.few ? 1 : (rows + 127) / 128) * (hd == 128 ? (Dv + 127) / 128 : 1);
-    const int64_t want = (pl.few ? 256 : 512) / (units < 1 ? 1 : units);
-    int64_t splits = want < 1 ? 1 : want;
-    const int64_t most = (Tk + 255) / 256;
-    if (splits > most) splits = most;
-    if (splits > 64) splits = 64;
-    const int64_t chunk = ((Tk + splits - 1) / splits + kt - 1) / kt * kt;
-    pl.chunk = (int)chunk;
-    pl.splits = (int)((Tk + chunk - 1) / chunk);
-    if (pl.splits < 1) pl.splits = 1;
+    if (pl.few) {
+        int64_t n = 256 / units, most = Tk > 255 * 64 ? 64 : (Tk + 255) / 256;
+        n = n < 1 ? 1 : (n < most ? n : most);
+        const int64_t chunk = ((Tk + n - 1) / n + 127) / 128 * 128;
+        pl.chunk = (int)chunk;
+        pl.splits = (int)((Tk + chunk - 1) / chunk);
+    } else {
+        int64_t chunk;
+        const int slots = 256 * (es == 4 ? (hd == 32 ? 2 : 1) : (hd == 32 ? 3 : (hd == 64 ? 2 : 1)));
+        pl.splits = diff_parts(units, slots, Tk, 64, es == 4 ? 6.0 * hd : 0.95 * hd, (double)B * Tq * H * (2 * Dv + 4) * 4, causal, chunk);
+        pl.chunk = (int)chunk;
+    }
     return pl;
 }
 
@@ -507,8 +538,12 @@ using namespace ndb;
 
 extern "C" int64_t nd_diff_attention_workspace_floats(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int dtype) {
     if (B <= 0 || Tq <= 0 || Tk <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || D > 128 || Dv <= 0 || Dv > 256) return -1;
-    const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv);
-    return pl.splits > 1 ? (int64_t)pl.splits * B * Tq * H * (2 * Dv + 4) : 0;
+    int splits = 1;
+    for (int causal = 0; causal < 2; ++causal) {
+        const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4, causal);
+        splits = pl.splits > splits ? pl.splits : splits;
+    }
+    return splits > 1 ? (int64_t)splits * B * Tq * H * (2 * Dv + 4) : 0;
 }
 
 extern "C" int nd_diff_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
@@ -527,7 +562,7 @@ extern "C" int nd_diff_attention(const void* q, int64_t q_sb, int64_t q_st, int6
     if (int rc = diff_check(fn, a, dtype)) return rc;
     a.g = H / Hk;
     NDB_REQUIRE(out && aligned_to(out, 16) && (!out1 || (out2 && lse && aligned_to(out1, 16) && aligned_to(out2, 16))), fn, "outputs missing or not 16-byte aligned");
-    const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv);
+    const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4, a.causal);
     a.splits = pl.splits, a.chunk = pl.chunk;
     NDB_REQUIRE(pl.splits == 1 || (workspace && aligned_to(workspace, 16)), fn, "workspace missing");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -14,6 +14,7 @@
 namespace ndb {
 
 int diff_head_dim(int D, int Dv);
+int diff_parts(int64_t units, int slots, int64_t length, int64_t grain, double per, double bytes, int causal, int64_t& share);
 int diff_check(const char* fn, const DiffArgs& a, int dtype);
 
 struct DiffBwdArgs {
@@ -194,7 +195,8 @@ __global__ void __launch_bounds__(64 * NW, (HD * (int)sizeof(T) == 64 ? 3 : (HD 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[m][e] = 0.f;
 #pragma unroll
-                for (int c = 0; c < S::NS; ++c) s[m] = mma_step<T>(TR::row(q32, rb, 0, m * S::PH + 2 * c), kf[m][c], s[m]);
+                for (int c = 0; c < S::NS; ++c)
+                    if (!no_step<T, HD>(c, f.D)) s[m] = mma_step<T>(TR::row(q32, rb, 0, m * S::PH + 2 * c), kf[m][c], s[m]);
             }
             // rows that see this lane's key: from `first` on (causal), no row past the last, none for a key past the sequence's end
             const int r_first = t0 + r32 + len - f.Tq;        // causal: the first row of the block sees the keys up to this one
@@ -220,13 +222,14 @@ __global__ void __launch_bounds__(64 * NW, (HD * (int)sizeof(T) == 64 ? 3 : (HD 
                 }
             }
             phase();
-            if constexpr (DVG) mma_cols<T, S::RB>(o32, cb, 0, 0, pd, dv);
+            if constexpr (DVG) mma_cols<T, S::RB>(o32, cb, 0, 0, f.Dv, pd, dv);
             if constexpr (DK) {
                 phase();
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dp[e] = 0.f;
 #pragma unroll
                 for (int c = 0; c < S::NSV; ++c) {
+                    if (no_step<T, HD>(c, f.Dv)) break;
                     u32x4 v;
                     if constexpr (S::V_LDS) v = TR::row(v_rows + wave * 32 * S::RB, rb, 0, 2 * c);
                     else v = vf[c];
@@ -245,7 +248,7 @@ __global__ void __launch_bounds__(64 * NW, (HD * (int)sizeof(T) == 64 ? 3 : (HD 
                         d2.set(e, lam * s[1][e] * (c2[j] - dp[e]));
                     }
                 }
-                mma_halves<T, S::RB, HD>(q32, cb, d1, d2, dk);
+                mma_halves<T, S::RB, HD>(q32, cb, f.D, d1, d2, dk);
             }
         }
         const bool through = c_t0 >= f.Tq;                    // this head's rows
@@ -387,12 +390,14 @@ __global__ void __launch_bounds__(256, (HD * (int)sizeof(T) >= 256 ? 1 : 2)) dif
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[m][e] = 0.f;
 #pragma unroll
-                for (int c = 0; c < S::NS; ++c) s[m] = mma_step<T>(TR::row(tk, rb, 0, m * S::PH + 2 * c), q[m][c], s[m]);
+                for (int c = 0; c < S::NS; ++c)
+                    if (!no_step<T, HD>(c, f.D)) s[m] = mma_step<T>(TR::row(tk, rb, 0, m * S::PH + 2 * c), q[m][c], s[m]);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) dp[e] = 0.f;
 #pragma unroll
-            for (int c = 0; c < S::NSV; ++c) dp = mma_step<T>(TR::row(tv, rb, 0, 2 * c), go[c], dp);
+            for (int c = 0; c < S::NSV; ++c)
+                if (!no_step<T, HD>(c, f.Dv)) dp = mma_step<T>(TR::row(tv, rb, 0, 2 * c), go[c], dp);
             const int left = seen - kb - 4 * lh;              // keys of this block the row sees
             if (f.causal ? kb + 32 > r0 / f.g + len - f.Tq + 1 : kb + 32 > len) {
 #pragma unroll
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(256, (HD * (int)sizeof(T) >= 256 ? 1 : 2)) dif
                 d1.set(e, p1 * (dp[e] - c1));
                 d2.set(e, nlam * p2 * (dp[e] - c2));
             }
-            mma_halves<T, S::RB, HD>(tk, cb, d1, d2, dq);
+            mma_halves<T, S::RB, HD>(tk, cb, f.D, d1, d2, dq);
         }
     };
     ring<2, decltype(lk)::NI + decltype(lv)::NI>(stages, STAGE, kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0, fetch, compute);
@@ -535,24 +540,21 @@ struct DiffBwdPlan {
 };
 
 // Rows of 256 bytes (D 33 .. 64 in bf16, to 32 in fp32): 8 waves share the rows that pass by, two to a SIMD in one workgroup a CU,
-// where that still fills the chip (8 x 2048^2 x 8 heads: 390 us for 440 with 4); others 4.  Fewer than 256 workgroups: their loops
-// are divided until about 512 exist, at least two tiles a share, and joined in order.
-static DiffBwdPlan diff_bwd_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int es) {
+// where that still fills the chip (8 x 2048^2 x 8 heads: 390 us for 440 with 4); others 4.  Loops divided as diff_parts says and
+// joined in order.
+static DiffBwdPlan diff_bwd_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int es, int causal) {
     DiffBwdPlan pl{};
     const int g = H / Hk;
     const int64_t units = (int64_t)B * Hk, rows = (int64_t)B * Tq * H, krows = (int64_t)B * Tk * Hk;
     pl.waves = diff_head_dim(D, Dv) * es == 128 && units * ((Tk + 255) / 256) >= 256 ? 8 : 4;
     pl.key_blocks = (Tk + 32 * pl.waves - 1) / (32 * pl.waves);
-    auto splits = [](int64_t blocks, int64_t most) {
-        int64_t n = blocks < 256 ? 512 / blocks : 1;
-        if (n > 16) n = 16;
-        if (n > most) n = most;
-        return (int)(n < 1 ? 1 : n);
-    };
-    pl.row_splits = splits(units * pl.key_blocks, (int64_t)g * ((Tq + 63) / 64) / 2);
-    pl.key_splits = splits(units * (((int64_t)Tq * g + 127) / 128), (Tk + 127) / 128);
-    pl.chunk = ((Tk + pl.key_splits - 1) / pl.key_splits + 63) / 64 * 64;
-    pl.key_splits = (Tk + pl.chunk - 1) / pl.chunk;
+    // a tile of rows (all heads of the group pass by) in the key kernel, 64 keys in the query kernel, in cycles per row / key
+    const int hd = diff_head_dim(D, Dv), rt = hd * es <= 64 * 2 ? 64 : 32;
+    int64_t share;
+    pl.row_splits = diff_parts(units * pl.key_blocks, 256 * (hd * es == 64 ? 3 : (hd * es == 128 && pl.waves == 4 ? 2 : 1)), (int64_t)g * ((Tq + rt - 1) / rt), 1,
+                               rt * (pl.waves / 4) * (es == 4 ? 12.0 : 2.0) * hd, (double)krows * (2 * D + Dv) * 4, causal, share);
+    pl.key_splits = diff_parts(units * (((int64_t)Tq * g + 127) / 128), hd * es >= 256 ? 256 : 512, Tk, 64, (es == 4 ? 8.0 : 1.3) * hd, (double)rows * 2 * D * 4, causal, share);
+    pl.chunk = (int)share;
     pl.dots = 2 * rows;
     pl.dlam = ((units * pl.key_blocks * pl.row_splits * pl.waves * g + H) + 3) / 4 * 4;
     pl.kv = pl.row_splits > 1 ? pl.row_splits * krows * (2 * D + Dv) : 0;
@@ -576,8 +578,13 @@ using namespace ndb;
 
 extern "C" int64_t nd_diff_attention_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int dtype) {
     if (B <= 0 || Tq <= 0 || Tk <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || D > 128 || Dv <= 0 || Dv > 256) return -1;
-    const DiffBwdPlan pl = diff_bwd_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4);
-    return pl.dots + pl.dlam + pl.kv + pl.q;
+    int64_t most = 0;
+    for (int causal = 0; causal < 2; ++causal) {
+        const DiffBwdPlan pl = diff_bwd_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4, causal);
+        const int64_t n = pl.dots + pl.dlam + pl.kv + pl.q;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 extern "C" int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
@@ -602,7 +609,7 @@ extern "C" int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, 
     NDB_REQUIRE(aligned_to(dout, 16) && do_sb % per == 0 && do_st % per == 0 && do_sh % per == 0 && do_st >= 0 && do_st <= (1 << 22), fn,
                 "rows of the output's gradient must be 16-byte aligned");
     NDB_REQUIRE(aligned_to(out1, 16) && aligned_to(out2, 16) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16), fn, "pointers must be 16-byte aligned");
-    const DiffBwdPlan pl = diff_bwd_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4);
+    const DiffBwdPlan pl = diff_bwd_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4, a.causal);
     p.waves = pl.waves, p.key_blocks = pl.key_blocks, p.row_splits = pl.row_splits, p.key_splits = pl.key_splits, p.chunk = pl.chunk;
     NDB_REQUIRE((int64_t)B * Hk * p.key_blocks <= (1 << 20) && (int64_t)B * Hk * (((int64_t)Tq * a.g + 127) / 128) <= (1 << 20), fn, "too many workgroups for one launch");
     NDB_REQUIRE(aligned_to(workspace, 16), fn, "workspace must be 16-byte aligned");
