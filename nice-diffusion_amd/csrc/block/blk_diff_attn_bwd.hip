@@ -9,6 +9,9 @@
 // in which dS is the next product's operand; the transposed operands are column reads of the same row-major tiles.
 // dlam is summed from fp32 P2 and dP, not from the rounded O2: it is one number and may cancel.  Rounding to bf16 besides the
 // outputs: P1 - lam P2, dS1, dS2 as operands, O1 and O2.  A sequence of one key has constant maps: dq and dk are made exactly zero.
+//
+// Measured, bf16, 8 x 2048^2 x 8 heads of 64 + 128, causal: D1 / D2 16 us, keys 250 us, queries 155 us (0.48 and 0.52 PFLOP/s of
+// matrix operations); what bounds them is what bounds the forward pass, with two exponentials and ~12 vector operations a score.
 #include "blk_diff_attn.h"
 
 namespace ndb {

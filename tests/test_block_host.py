@@ -75,7 +75,7 @@ def diff_args(**kw):
 
 
 @pytest.mark.parametrize('kw,what', [
-    (dict(Tk=0), 'positive'), (dict(H=3), 'multiple'), (dict(H=130), '64'), (dict(D=36), 'multiple of 8'), (dict(D=136), '128'), (dict(Dv=12), 'value dim'),
+    (dict(Tk=0), 'positive'), (dict(H=3), 'multiple'), (dict(H=130), '64'), (dict(H=1 << 21, Hk=1 << 21), 'heads'), (dict(D=36), 'multiple of 8'), (dict(D=136), '128'), (dict(Dv=12), 'value dim'),
     (dict(Dv=264), '256'), (dict(Tq=1 << 29, H=2), 'tokens'), (dict(scale=0.0), 'scale'), (dict(scale=float('nan')), 'scale'), (dict(k=None), 'null'),
     (dict(k=A + 8), 'aligned'), (dict(vs=(640, 132, 64)), 'aligned'), (dict(qs=(640, 1 << 23, 64)), 'stride'), (dict(ks=(640, -128, 64)), 'stride'),
     (dict(lam=(A, A, None, A)), 'lambda'), (dict(out=None), 'outputs'), (dict(o1=A), 'outputs'), (dict(Tk=1 << 20, B=1, Tq=1, ws=None), 'workspace'),
