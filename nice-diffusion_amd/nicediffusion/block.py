@@ -91,7 +91,8 @@ def _aligned(t):
     """A contiguous parameter on a 16-byte boundary."""
     if t is None:
         return None
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -137,23 +138,27 @@ def rotary_table(positions, channels, theta=10000.0):
 
 
 def _table(t, name, B, T):
-    if t.dtype != torch.float32:
+    """A table [T, pairs] or [1 or B, T, pairs] with contiguous token rows (the batch may have a stride of its own)."""
+    if t.dtype is not torch.float32:
         raise TypeError('{} is {}: float32 tables expected'.format(name, t.dtype))
     if t.requires_grad:
         raise ValueError('{} requires a gradient: the tables are constants'.format(name))
-    if t.dim() == 2:
-        t = t[None]
-    if t.dim() != 3 or t.shape[0] not in (1, B) or t.shape[1] != T:
-        raise ValueError('{} has shape {}, expected [{}, pairs] or [{}, {}, pairs]'.format(name, tuple(t.shape), T, B, T))
-    if t.stride(2) != 1 or t.stride(1) != t.shape[2]:
-        t = t.contiguous()
-    return t
+    shape = t.shape
+    n = len(shape)
+    if n not in (2, 3) or shape[n - 2] != T or (n == 3 and shape[0] not in (1, B)):
+        raise ValueError('{} has shape {}, expected [{}, pairs] or [{}, {}, pairs]'.format(name, tuple(shape), T, B, T))
+    if t.is_contiguous():
+        return t
+    return t if t.stride(-1) == 1 and t.stride(-2) == shape[-1] else t.contiguous()
+
+
+def _table_stride(t):
+    return t.stride(0) if t is not None and t.dim() == 3 and t.shape[0] > 1 else 0
 
 
 def _launch_qk(q, k, qw, kw, cos, sin, eps, interleaved, qo, ko):
     B, T, Hq, D = q.shape
-    R = 0 if cos is None else 2 * cos.shape[-1]
-    tb = 0 if cos is None or cos.shape[0] == 1 else cos.stride(0)
+    R, tb = 0 if cos is None else 2 * cos.shape[-1], _table_stride(cos)
     _call('nd_qk_norm_rope', q.device, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), _hip.ptr(qw), _hip.ptr(kw), _hip.ptr(cos),
           _hip.ptr(sin), tb, qo.data_ptr(), *_strides(qo), ko.data_ptr(), *_strides(ko), B, T, Hq, k.shape[2], D, R, eps,
           _hip.ROPE_INTERLEAVED if interleaved else 0, _DT[q.dtype])
@@ -184,8 +189,7 @@ class _QkNormRope(torch.autograd.Function):
             if dqw is not None or dkw is not None:
                 n = _hip.load_block().nd_qk_norm_rope_bwd_workspace_floats(B, T, Hq, Hk, D)
                 ws = torch.empty(n, dtype=torch.float32, device=q.device)
-            R = 0 if cos is None else 2 * cos.shape[-1]
-            tb = 0 if cos is None or cos.shape[0] == 1 else cos.stride(0)
+            R, tb = 0 if cos is None else 2 * cos.shape[-1], _table_stride(cos)
             _call('nd_qk_norm_rope_bwd', q.device, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), _hip.ptr(qw), _hip.ptr(kw),
                   _hip.ptr(cos), _hip.ptr(sin), tb, dqo.data_ptr(), *_strides(dqo), dko.data_ptr(), *_strides(dko), dq.data_ptr(),
                   *_strides(dq), dk.data_ptr(), *_strides(dk), _hip.ptr(dqw), _hip.ptr(dkw), _hip.ptr(ws), B, T, Hq, Hk, D, R, ctx.eps,
@@ -218,10 +222,10 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
         raise ValueError('q and k need at least one head')
     if q_weight is not None:
         _shape(q_weight, 'q_weight', D)
-        q_weight = q_weight.contiguous()
+        q_weight = _aligned(q_weight)
     if k_weight is not None:
         _shape(k_weight, 'k_weight', D)
-        k_weight = k_weight.contiguous()
+        k_weight = _aligned(k_weight)
     if (cos is None) != (sin is None):
         raise ValueError('cos and sin come together')
     if cos is not None:
@@ -230,7 +234,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
         if cos.shape != sin.shape:
             raise ValueError('cos has shape {}, sin {}'.format(tuple(cos.shape), tuple(sin.shape)))
         cos, sin = _table(cos, 'cos', B, T), _table(sin, 'sin', B, T)
-        if cos.shape[0] > 1 and cos.stride(0) != sin.stride(0):
+        if _table_stride(cos) != _table_stride(sin):
             cos, sin = cos.contiguous(), sin.contiguous()
         if not 0 < 2 * cos.shape[-1] <= D:
             raise ValueError('tables for {} channels, head dim is {}'.format(2 * cos.shape[-1], D))
@@ -389,10 +393,10 @@ def _ld(m):
     return m.shape[1] if m.shape[0] == 1 else m.stride(0)
 
 
-def _launch_ffn(x, w_in, b_in, w_out, b_out, res, act, keep):
+def _launch_ffn(x, w_in, b_in, w_out, b_out, res, act, keep, shape):
     M, C = x.shape
     F = w_out.shape[1]
-    y, h = x.new_empty(M, C), x.new_empty(M, F)
+    y, h = x.new_empty(shape), x.new_empty(M, F)
     au = x.new_empty(M, 2 * F) if keep else None
     ws = _floats(_hip.load_block().nd_gated_ffn_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
     _call('nd_gated_ffn', x.device, x.data_ptr(), _ld(x), w_in.data_ptr(), _hip.ptr(b_in), w_out.data_ptr(), _hip.ptr(b_out), _hip.ptr(res),
@@ -405,14 +409,14 @@ class _GatedFfn(torch.autograd.Function):
     def forward(ctx, x, w_in, b_in, w_out, b_out, res, act):
         C = x.shape[-1]
         xm, wi, wo = _matrix(x, C), _aligned(w_in), _aligned(w_out)
-        rm = None if res is None else _matrix(res, C)
+        rm = xm if res is x else (None if res is None else _matrix(res, C))
         if xm.shape[0]:
-            y, h, au = _launch_ffn(xm, wi, _aligned(b_in), wo, _aligned(b_out), rm, act, True)
+            y, h, au = _launch_ffn(xm, wi, _aligned(b_in), wo, _aligned(b_out), rm, act, True, x.shape)
         else:
-            y, h, au = xm.new_empty(0, C), None, None
+            y, h, au = xm.new_empty(x.shape), None, None
         ctx.save_for_backward(xm, wi, wo, h, au)
         ctx.act, ctx.shape = act, x.shape
-        return y.view(x.shape)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -477,5 +481,6 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, residual=None, act
         return _GatedFfn.apply(x, w_in, b_in, w_out, b_out, residual, act)
     if x.numel() == 0:
         return torch.empty_like(x, memory_format=torch.contiguous_format)
-    res = None if residual is None else _matrix(residual, C)
-    return _launch_ffn(_matrix(x, C), _aligned(w_in), _aligned(b_in), _aligned(w_out), _aligned(b_out), res, act, False)[0].view(x.shape)
+    xm = _matrix(x, C)
+    res = xm if residual is x else (None if residual is None else _matrix(residual, C))
+    return _launch_ffn(xm, _aligned(w_in), _aligned(b_in), _aligned(w_out), _aligned(b_out), res, act, False, x.shape)[0]
