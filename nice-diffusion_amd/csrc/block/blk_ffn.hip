@@ -210,17 +210,33 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const float* part, int s
     }
 }
 
-// column sums of src [M, N]: 8 columns a thread, 8 rows side by side a block; partial row per block, then the rows in order
+// Column sums of one or two matrices [M, N] at once: 8 columns a thread, 8 rows side by side a block; a partial row per block, then
+// the rows in order.  (Both bias gradients in two launches instead of four:
+// 139 us for 147 at 2355 x 264 x 680 in fp32, with all gradients.)
 template <typename T>
-__global__ void __launch_bounds__(256) colsum_kernel(const T* src, int64_t ld, int M, int N, float* part) {
+struct ColSum {
+    const T* src;
+    int64_t ld;
+    int N, rows;              // columns, row blocks
+    float* part;              // [rows][N]
+    T* out;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) colsum_kernel(const ColSum<T> first, const ColSum<T> second, int M) {
     __shared__ float red[8][257];
-    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, n = (blockIdx.x * 32 + cx) * 8;
+    const int blocks = (first.N + 255) / 256;
+    const bool other = (int)blockIdx.x >= blocks;
+    const ColSum<T>& p = other ? second : first;
+    if ((int)blockIdx.y >= p.rows) return;
+    const int bx = other ? blockIdx.x - blocks : blockIdx.x;
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, n = (bx * 32 + cx) * 8;
     float s[8] = {};
-    if (n < N) {
+    if (n < p.N) {
 #pragma unroll 4
-        for (int m = blockIdx.y * 8 + ry; m < M; m += gridDim.y * 8) {
+        for (int m = blockIdx.y * 8 + ry; m < M; m += p.rows * 8) {
             float v[8];
-            load_vec<T, 8>(src + m * ld + n, v);
+            load_vec<T, 8>(p.src + m * p.ld + n, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
@@ -228,28 +244,31 @@ __global__ void __launch_bounds__(256) colsum_kernel(const T* src, int64_t ld, i
 #pragma unroll
     for (int e = 0; e < 8; ++e) red[ry][cx * 8 + e] = s[e];
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c < N) {
+    const int c = bx * 256 + threadIdx.x;
+    if (c < p.N) {
         float t = 0.f;
 #pragma unroll
         for (int r = 0; r < 8; ++r) t += red[r][threadIdx.x];
-        part[(int64_t)blockIdx.y * N + c] = t;
+        p.part[(int64_t)blockIdx.y * p.N + c] = t;
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(1024) colsum_join_kernel(const float* part, int rows, int N, T* out) {
+__global__ void __launch_bounds__(1024) colsum_join_kernel(const ColSum<T> first, const ColSum<T> second) {
     __shared__ float red[32][33];
-    const int n = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+    const int blocks = (first.N + 31) / 32;
+    const bool other = (int)blockIdx.x >= blocks;
+    const ColSum<T>& p = other ? second : first;
+    const int n = (other ? blockIdx.x - blocks : blockIdx.x) * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
     float t = 0.f;
-    if (n < N)
-        for (int r = lane; r < rows; r += 32) t += part[(int64_t)r * N + n];
+    if (n < p.N)
+        for (int r = lane; r < p.rows; r += 32) t += p.part[(int64_t)r * p.N + n];
     red[lane][threadIdx.x & 31] = t;
     __syncthreads();
-    if (lane == 0 && n < N) {
+    if (lane == 0 && n < p.N) {
         float u = 0.f;
         for (int l = 0; l < 32; ++l) u += red[l][threadIdx.x & 31];
-        out[n] = (T)u;
+        p.out[n] = (T)u;
     }
 }
 
@@ -446,10 +465,10 @@ static int colsum_blocks(int64_t M, int64_t N) {
 }
 
 template <typename T>
-static int run_colsum(const char* fn, const T* src, int64_t ld, int M, int N, float* ws, T* out, hipStream_t st) {
-    const int rb = colsum_blocks(M, N);
-    hipLaunchKernelGGL((colsum_kernel<T>), dim3((N + 255) / 256, rb), dim3(256), 0, st, src, ld, M, N, ws);
-    hipLaunchKernelGGL((colsum_join_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, ws, rb, N, out);
+static int run_colsum(const char* fn, const ColSum<T>& first, const ColSum<T>& second, int M, hipStream_t st) {
+    const int rows = first.rows > second.rows ? first.rows : second.rows;
+    hipLaunchKernelGGL((colsum_kernel<T>), dim3((first.N + 255) / 256 + (second.N + 255) / 256, rows), dim3(256), 0, st, first, second, M);
+    hipLaunchKernelGGL((colsum_join_kernel<T>), dim3((first.N + 31) / 32 + (second.N + 31) / 32), dim3(1024), 0, st, first, second);
     return check_launch(fn);
 }
 
@@ -506,10 +525,11 @@ static int ffn_backward(const char* fn, const FfnBwd<T>& a, hipStream_t st) {
         if (int rc = run_gemm_out<T, false, false>(fn, GemmSide<T>{a.dy, a.lddy, C}, GemmSide<T>{a.h, F, F}, M, a.ws,
                                                    EpiOut<T>{nullptr, nullptr, a.dw_out, 0, F}, st))
             return rc;
-    if (a.db_in)
-        if (int rc = run_colsum<T>(fn, a.dau, 2 * F, M, 2 * F, a.ws, a.db_in, st)) return rc;
-    if (a.db_out)
-        if (int rc = run_colsum<T>(fn, a.dy, a.lddy, M, C, a.ws, a.db_out, st)) return rc;
+    if (a.db_in || a.db_out) {
+        ColSum<T> in{a.dau, 2 * F, a.db_in ? 2 * F : 0, a.db_in ? colsum_blocks(M, 2 * F) : 0, a.ws, a.db_in};
+        ColSum<T> out{a.dy, a.lddy, a.db_out ? C : 0, a.db_out ? colsum_blocks(M, C) : 0, a.ws + (int64_t)in.rows * in.N, a.db_out};
+        if (int rc = run_colsum<T>(fn, in, out, M, st)) return rc;
+    }
     return ND_OK;
 }
 
@@ -559,8 +579,8 @@ extern "C" int64_t nd_gated_ffn_bwd_workspace_floats(int M, int C, int F, int dt
     if (M <= 0 || C <= 0 || F <= 0) return -1;
     const int es = dtype == ND_DT_BF16 ? 2 : 4;
     int64_t n = split_floats(M, C, 2LL * F, es);
-    const int64_t more[4] = {split_floats(2LL * F, C, M, es), split_floats(C, F, M, es), (int64_t)colsum_blocks(M, 2LL * F) * 2 * F,
-                             (int64_t)colsum_blocks(M, C) * C};
+    const int64_t more[3] = {split_floats(2LL * F, C, M, es), split_floats(C, F, M, es),
+                             (int64_t)colsum_blocks(M, 2LL * F) * 2 * F + (int64_t)colsum_blocks(M, C) * C};
     for (int64_t v : more) n = v > n ? v : n;
     return n;
 }
