@@ -13,18 +13,15 @@
 //              LDS.  bf16, 8 x 2048^2 x 8 heads of 64 + 128: 217 us (0.95 PFLOP/s of matrix operations), causal 130; 64 x 1024^2 x 6
 //              heads of 32 + 64: 212 us.  Bound by the SIMD's issue: matrix operations and the softmax's vector operations add up
 //              rather than overlap (a fused multiply-add 2.5 cycles beside them, an exponential 2.8 to 8)
-//   few rows   (g Tq <= 32: single tokens) a read of the cache: 8 waves (fewer for wide tiles) share the rows, each with a tile of
-//              32 keys of its own, no barrier; the next keys are requested when the scores are made, the next values when the
-//              outputs are, so about 3/4 of 128 KiB a CU is under way.  16 x 16 heads (4 key heads), 64 + 128 channels, ragged
-//              caches up to 8192 (197 MB): 51 us; tiles of 128 keys for the whole workgroup in two stages 62, four 32-key
-//              stages for each of 2 waves 81
+//   few rows   (g Tq <= 32: single tokens) a kernel of its own: diff_few_kernel
 //   wide heads (D > 64) 128 value channels a workgroup, the scores made twice when Dv is above that: both maps' outputs and the
 //              queries of 256 channels do not fit the registers (measured: 290 spilled)
 //   splits     when (batch, key head, row tile) does not fill the chip the keys are divided over workgroups; fp32 partial
 //              outputs, joined in split order by a second launch
 // No maximum is taken of a tile as a rule: its weights are made against the row's reference of before, and only where their sum
 // passes 2^10 (or nothing was seen so far) the reference moves to the tile's maximum and they are made again: a weight stays
-// below 2^10, as exact in floating point as one below 1.  Rounding to bf16 besides the output: the weights p as the second product's operand; their sum is taken from the rounded values.
+// below 2^10, as exact in floating point as one below 1.  Rounding to bf16 besides the output: the weights p as the second product's
+// operand; their sum is taken from the rounded values.
 #include "blk_diff_attn.h"
 
 namespace ndb {
@@ -40,11 +37,7 @@ struct DiffShape {
     // few rows: each wave has a tile of 32 keys of its own, up to 128 KiB together
     static constexpr int TILE_FEW = 32 * (RBK + RBV);
     static constexpr int NW_FEW = TILE_FEW <= 16384 ? 8 : (TILE_FEW <= 32768 ? 4 : 2);
-    static constexpr int DP_FEW = TILE_FEW >= 16384 ? 2 : 1;  // 32-channel blocks of both maps joined at a time
 };
-
-template <typename T, int HD, bool FEW>
-constexpr int diff_threads() { return FEW ? 64 * DiffShape<T, HD>::NW_FEW : 256; }
 
 // four channels dd .. of output row `orow` from both maps' sums and their statistics (maximum, sum of weights, twice)
 template <typename T>
@@ -68,30 +61,23 @@ __device__ __forceinline__ void diff_store(const DiffArgs& p, int64_t orow, int 
     }
 }
 
-template <typename T, int HD, bool FEW>
-__global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeof(T) >= 256 ? 1 : (HD == 32 && sizeof(T) == 2 && !FEW ? 3 : 2))) diff_attn_kernel(const DiffArgs p) {
+template <typename T, int HD>
+__global__ void __launch_bounds__(256, (HD * (int)sizeof(T) >= 256 ? 1 : (HD == 32 && sizeof(T) == 2 ? 3 : 2))) diff_attn_kernel(const DiffArgs p) {
     using S = DiffShape<T, HD>;
-    constexpr int KT = FEW ? 32 : S::KT_MANY;                // keys of a tile
-    constexpr int NW = FEW ? S::NW_FEW : 4;                  // waves
+    constexpr int KT = S::KT_MANY, NW = 4;                    // keys of a tile, waves
     constexpr int NJ = 1;                                     // 32-key blocks at a time (2 at D <= 32: 181 registers for 142, no faster)
     constexpr int STAGE = KT * (S::RBK + S::RBV);
-    constexpr int NST = HD == 32 && S::ES == 2 ? 3 : 2;       // tiles in LDS (few rows: one a wave)
-    constexpr int LDS = STAGE * (FEW ? NW : NST);
+    constexpr int NST = HD == 32 && S::ES == 2 ? 3 : 2;       // tiles in LDS
     using TK = Tile<T, S::RBK>;
     using TV = Tile<T, S::RBV>;
-    static_assert(!FEW || S::DP_FEW * 8192 <= STAGE, "a wave's part of the join fits its tile");
-    __shared__ __attribute__((aligned(16))) char stages[LDS];
+    __shared__ __attribute__((aligned(16))) char stages[NST * STAGE];
     __shared__ float lam_s[DIFF_MAX_GROUP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, lh = lane >> 5;
 
-    const int rows = p.Tq * p.g, tiles = (rows + (FEW ? 31 : 127)) / (FEW ? 32 : 128);
+    const int rows = p.Tq * p.g, tiles = (rows + 127) / 128;
     int bh, id;
-    if (FEW) {                                                // nothing to share: the (batch, key head)s in turn, so that every XCD
-        id = blockIdx.x / (p.B * p.Hk), bh = blockIdx.x - id * (p.B * p.Hk);      // has long and short sequences
-    } else {
-        unit_of(blockIdx.x, gridDim.x, p.B * p.Hk, p.causal, bh, id);
-    }
+    unit_of(blockIdx.x, gridDim.x, p.B * p.Hk, p.causal, bh, id);
     const int vb = HD == 128 ? id / (tiles * p.splits) : 0, dv0 = vb * S::DV, dvn = p.Dv - dv0 < S::DV ? p.Dv - dv0 : S::DV;
     id -= vb * tiles * p.splits;
     const int sp = id / tiles, tile = tiles - 1 - (id - sp * tiles);      // longest rows first
@@ -99,13 +85,13 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
     const int len = diff_length(p.lengths, b, p.Tk);
 
     // this lane's row
-    const int r0 = tile * (FEW ? 32 : 128) + (FEW ? 0 : wave * 32);
+    const int r0 = tile * 128 + wave * 32;
     const int r = r0 + l31 < rows ? r0 + l31 : rows - 1;
     const int t = r / p.g, hg = r - t * p.g, head = hk * p.g + hg;
     const int seen = p.causal ? t + len - p.Tq + 1 : len;      // keys this row sees (<= 0: none)
     int last = len;                                            // keys the workgroup needs
     if (p.causal) {
-        const int rl = (tile + 1) * (FEW ? 32 : 128) - 1 < rows ? (tile + 1) * (FEW ? 32 : 128) - 1 : rows - 1;
+        const int rl = (tile + 1) * 128 - 1 < rows ? (tile + 1) * 128 - 1 : rows - 1;
         last = rl / p.g + len - p.Tq + 1;
     }
     const int kbeg = sp * p.chunk;
@@ -138,31 +124,21 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
             for (int e = 0; e < 16; ++e) o[m][d][e] = 0.f;
     float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    TileLoad<T, S::RBK, KT, FEW ? 1 : NW> lk;
-    TileLoad<T, S::RBV, KT, FEW ? 1 : NW> lv;
-    const int lw = FEW ? 0 : wave;
-    lk.template init<S::RBK / 2>(p.k.st * S::ES, p.D * S::ES, lw, lane);
-    lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, lw, lane);
-    const int tile_step = FEW ? KT * NW : KT, kfirst = FEW ? kbeg + wave * KT : kbeg;      // few rows: the waves take tiles in turn
+    TileLoad<T, S::RBK, KT, NW> lk;
+    TileLoad<T, S::RBV, KT, NW> lv;
+    lk.template init<S::RBK / 2>(p.k.st * S::ES, p.D * S::ES, wave, lane);
+    lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, wave, lane);
     const T* kp = static_cast<const T*>(p.k.p) + b * p.k.sb + hk * p.k.sh;
     const T* vp = static_cast<const T*>(p.v.p) + b * p.v.sb + hk * p.v.sh + dv0;
-    auto fetch_k = [&](int i, char* at) {                     // keys at or past the sequence's end become zero rows
-        const int key = kfirst + i * tile_step;
+    auto fetch = [&](int i, char* at) {                       // keys at or past the sequence's end become zero rows
+        const int key = kbeg + i * KT;
         const int64_t n = len - key;
-        lk.load(at, kp + (int64_t)key * p.k.st, ((n - 1) * p.k.st + 2 * p.D) * S::ES, lw);
-    };
-    auto fetch_v = [&](int i, char* at) {
-        const int key = kfirst + i * tile_step;
-        const int64_t n = len - key;
-        lv.load(at + KT * S::RBK, vp + (int64_t)key * p.v.st, ((n - 1) * p.v.st + dvn) * S::ES, lw);
-    };
-    auto fetch = [&](int i, char* at) {
-        fetch_k(i, at);
-        fetch_v(i, at);
+        lk.load(at, kp + (int64_t)key * p.k.st, ((n - 1) * p.k.st + 2 * p.D) * S::ES, wave);
+        lv.load(at + KT * S::RBK, vp + (int64_t)key * p.v.st, ((n - 1) * p.v.st + dvn) * S::ES, wave);
     };
     const int row_base = TK::row_base(lane), col_base = TV::col_base(lane);
-    auto compute = [&](int i, const char* tk, auto&& scored) {       // scored(): the tile's keys are read
-        const int key0 = kfirst + i * tile_step;
+    auto compute = [&](int i, const char* tk) {
+        const int key0 = kbeg + i * KT;
         const char* tv = tk + KT * S::RBK;
 #pragma unroll 1
         for (int sub = 0; sub < KT / 32; sub += NJ) {
@@ -182,7 +158,6 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
                     for (int c = 0; c < S::NS; ++c)
                         if (!no_step<T, HD>(c, p.D)) s[m][j] = mma_step<T>(TK::row(k32, rb, 32 * j, m * S::PH + 2 * c), q[m][c], s[m][j]);
                 }
-            scored();
             // scores past what a row sees: only in the tile that holds a row's end
             const bool cut = p.causal ? kb + 32 * NJ > r0 / p.g + len - p.Tq + 1 : kb + 32 * NJ > len;
             if (cut) {
@@ -265,99 +240,11 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
             }
         }
     };
-    const int n = kend > kfirst ? (kend - kfirst + tile_step - 1) / tile_step : 0;
-    if constexpr (FEW) {                                      // the next tile's keys after the scores, its values after the outputs
-        constexpr int NK = decltype(lk)::NI, NV = decltype(lv)::NI;
-        char* mine = stages + wave * STAGE;
-        if (n > 0) fetch(0, mine);
-        for (int i = 0; i < n; ++i) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV) : "memory");      // the tile's keys are there ...
-            compute(i, mine, [&] {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (i + 1 < n) {
-                    fetch_k(i + 1, mine);
-                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK) : "memory");      // ... and its values
-                } else {
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                }
-            });
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (i + 1 < n) fetch_v(i + 1, mine);
-        }
-    } else {
-        ring<NST, decltype(lk)::NI + decltype(lv)::NI>(stages, STAGE, n, fetch, [&](int i, const char* at) { compute(i, at, [] {}); });
-    }
+    ring<NST, decltype(lk)::NI + decltype(lv)::NI>(stages, STAGE, kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0, fetch, compute);
     l[0] = half_sum(l[0]);
     l[1] = half_sum(l[1]);
     __syncthreads();                                          // lam_s is written; the stages are free
 
-    if constexpr (FEW) {                                      // join the waves
-        __shared__ float ml[NW][32][4];
-        if (lh == 0) {
-            ml[wave][l31][0] = mx[0];
-            ml[wave][l31][1] = l[0];
-            ml[wave][l31][2] = mx[1];
-            ml[wave][l31][3] = l[1];
-        }
-        __syncthreads();
-        float f[2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {                         // a common maximum
-            float top = -INFINITY, sum = 0.f;
-            for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][l31][2 * m]);
-            const float ref = top == -INFINITY ? 0.f : top;
-            for (int w = 0; w < NW; ++w) sum += ml[w][l31][2 * m + 1] * __builtin_amdgcn_exp2f(ml[w][l31][2 * m] - ref);
-            f[m] = __builtin_amdgcn_exp2f(mx[m] - ref);
-            mx[m] = top;
-            l[m] = sum;
-        }
-        __syncthreads();
-        if (wave == 0 && lh == 0) {
-            ml[0][l31][0] = mx[0];
-            ml[0][l31][1] = l[0];
-            ml[0][l31][2] = mx[1];
-            ml[0][l31][3] = l[1];
-        }
-        // then the outputs, DP blocks of 32 channels of both maps at a time: added in wave order, each element by one thread
-        constexpr int DP = S::DP_FEW, PC = DP * 8;            // 16-byte pieces of a row and map
-#pragma unroll
-        for (int d0 = 0; d0 < S::NDT; d0 += DP) {
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int d = 0; d < DP; ++d)
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) {
-                        const f32x16& x = o[m][d0 + d];
-                        const int pc = (m * DP + d) * 8 + 2 * g4 + lh;
-                        *reinterpret_cast<f32x4*>(stages + (wave * 32 + l31) * (2 * PC * 16) + ((pc ^ (l31 & 7)) << 4)) =
-                            f32x4{x[4 * g4] * f[m], x[4 * g4 + 1] * f[m], x[4 * g4 + 2] * f[m], x[4 * g4 + 3] * f[m]};
-                    }
-            __syncthreads();
-            for (int e = threadIdx.x; e < rows * PC; e += NW * 64) {
-                const int row = e / PC, pc = e - row * PC, dd = d0 * 32 + pc * 4;
-                if (dd >= dvn) continue;
-                f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                for (int w = 0; w < NW; ++w)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-                        sum[m] += *reinterpret_cast<const f32x4*>(stages + (w * 32 + row) * (2 * PC * 16) + (((m * PC + pc) ^ (row & 7)) << 4));
-                const f32x4 st = *reinterpret_cast<const f32x4*>(ml[0][row]);
-                const bool first = dd == 0 && vb == 0;
-                if (p.splits > 1) {
-                    float* at = p.part + ((int64_t)sp * p.B * p.Hk * rows + (int64_t)bh * rows + row) * (2 * p.Dv + 4);
-                    *reinterpret_cast<f32x4*>(at + dv0 + dd) = sum[0];
-                    *reinterpret_cast<f32x4*>(at + p.Dv + dv0 + dd) = sum[1];
-                    if (first) *reinterpret_cast<f32x4*>(at + 2 * p.Dv) = st;
-                    continue;
-                }
-                const int tt = row / p.g, h = row - tt * p.g;
-                diff_store<T>(p, ((int64_t)b * p.Tq + tt) * p.H + hk * p.g + h, dv0 + dd, sum, st, lam_s[h], first);
-            }
-            __syncthreads();
-        }
-        return;
-    }
     if (r0 + l31 >= rows) return;
     if (p.splits > 1) {
         float* at = p.part + ((int64_t)sp * p.B * p.Hk * rows + (int64_t)bh * rows + r) * (2 * p.Dv + 4);
@@ -388,48 +275,266 @@ __global__ void __launch_bounds__((diff_threads<T, HD, FEW>()), (HD * (int)sizeo
         }
 }
 
-// joins the splits of a row: Dv / 4 threads a row
+// Few rows: a read of the cache.  8 waves (fewer for wide tiles), each with a tile of 32 keys of its own, no barrier; the next keys
+// are requested when the scores are made, the next values when the outputs are, so about 3/4 of 128 KiB a CU is under way.
+// A row's two maps are two columns of the products (column 16 m + row: 16 rows a workgroup), so one exponential a key and lane and
+// one product with the values serve both; the scores are made with either half of the keys, and a lane takes those of its own map.
+// What the bf16 weights leave out is a second bf16 operand here (49.3 us becomes 50.0, and the error is the output's rounding alone).
+// 16 tokens, 16 heads on 4, 64 + 128 channels, ragged caches up to 8192 (197 MB, 38 us as a copy): 48.5 us with the join; with 128-key
+// tiles for the whole workgroup in two stages 62, four 32-key stages for each of 2 waves 81, accumulators for either map 51.
+template <typename T, int HD>
+__global__ void __launch_bounds__((64 * DiffShape<T, HD>::NW_FEW), (HD * (int)sizeof(T) >= 256 ? 1 : 2)) diff_few_kernel(const DiffArgs p) {
+    using S = DiffShape<T, HD>;
+    using TK = Tile<T, S::RBK>;
+    using TV = Tile<T, S::RBV>;
+    constexpr int NW = S::NW_FEW, STAGE = S::TILE_FEW;
+    constexpr bool REST = S::ES == 2;
+    static_assert(S::NDT * 4096 <= STAGE, "a wave's part of the join fits its tile");
+    __shared__ __attribute__((aligned(16))) char stages[NW * STAGE];
+    __shared__ float ml[NW][32][2], lam_s[DIFF_MAX_GROUP];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, lh = lane >> 5, map = l31 >> 4;
+
+    // nothing to share: the (batch, key head)s in turn, so that every XCD has long and short sequences
+    const int rows = p.Tq * p.g, tiles = (rows + 15) / 16;
+    int id = blockIdx.x / (p.B * p.Hk);
+    const int bh = blockIdx.x - id * (p.B * p.Hk);
+    const int vb = HD == 128 ? id / (tiles * p.splits) : 0, dv0 = vb * S::DV, dvn = p.Dv - dv0 < S::DV ? p.Dv - dv0 : S::DV;
+    id -= vb * tiles * p.splits;
+    const int sp = id / tiles, tile = id - sp * tiles;
+    const int b = bh / p.Hk, hk = bh - b * p.Hk;
+    const int len = diff_length(p.lengths, b, p.Tk);
+
+    const int r0 = tile * 16, r = r0 + (l31 & 15) < rows ? r0 + (l31 & 15) : rows - 1;
+    const int t = r / p.g, hg = r - t * p.g;
+    const int seen = p.causal ? t + len - p.Tq + 1 : len;      // keys this row sees (<= 0: none)
+    const int cut_from = p.causal ? r0 / p.g + len - p.Tq + 1 : len;      // keys from here on are not seen by every row
+    const int rl = r0 + 15 < rows ? r0 + 15 : rows - 1;
+    const int last = p.causal ? rl / p.g + len - p.Tq + 1 : len;
+    const int kbeg = sp * p.chunk, kend = kbeg + p.chunk < last ? kbeg + p.chunk : last;
+
+    for (int h = wave; h < (p.splits == 1 ? p.g : 0); h += NW) {      // divided keys: the join makes them
+        float e1, e2;
+        diff_lambda<T>(p, hk * p.g + h, lane, e1, e2);
+        if (lane == 0) lam_s[h] = e1 - e2 + p.lam_init;
+    }
+    u32x4 q[S::NS];
+    {
+        const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q.p) + b * p.q.sb + t * p.q.st + (hk * p.g + hg) * p.q.sh + map * p.D);
+#pragma unroll
+        for (int c = 0; c < S::NS; ++c) {
+            const int by = (2 * c + lh) * 16;
+            q[c] = u32x4{0u, 0u, 0u, 0u};
+            if (by < p.D * S::ES) q[c] = *reinterpret_cast<const u32x4*>(qp + by);
+        }
+    }
+    f32x16 o[S::NDT];
+#pragma unroll
+    for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+
+    TileLoad<T, S::RBK, 32, 1> lk;
+    TileLoad<T, S::RBV, 32, 1> lv;
+    lk.template init<S::RBK / 2>(p.k.st * S::ES, p.D * S::ES, 0, lane);
+    lv.template init<S::RBV>(p.v.st * S::ES, dvn * S::ES, 0, lane);
+    const T* kp = static_cast<const T*>(p.k.p) + b * p.k.sb + hk * p.k.sh;
+    const T* vp = static_cast<const T*>(p.v.p) + b * p.v.sb + hk * p.v.sh + dv0;
+    char* const tk = stages + wave * STAGE;
+    char* const tv = tk + 32 * S::RBK;
+    const int first = kbeg + wave * 32, n = kend > first ? (kend - first + 32 * NW - 1) / (32 * NW) : 0;      // the waves take tiles in turn
+    auto fetch_k = [&](int i) {                               // keys at or past the sequence's end become zero rows
+        const int key = first + i * 32 * NW;
+        lk.load(tk, kp + (int64_t)key * p.k.st, ((int64_t)(len - key - 1) * p.k.st + 2 * p.D) * S::ES, 0);
+    };
+    auto fetch_v = [&](int i) {
+        const int key = first + i * 32 * NW;
+        lv.load(tv, vp + (int64_t)key * p.v.st, ((int64_t)(len - key - 1) * p.v.st + dvn) * S::ES, 0);
+    };
+    constexpr int NK = decltype(lk)::NI, NV = decltype(lv)::NI;
+    const int row_base = TK::row_base(lane), col_base = TV::col_base(lane);
+    if (n > 0) {
+        fetch_k(0);
+        fetch_v(0);
+    }
+    for (int i = 0; i < n; ++i) {
+        const int kb = first + i * 32 * NW;
+        const int rb = in_loop(row_base), cb = in_loop(col_base);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV) : "memory");      // the tile's keys are there
+        f32x16 s, s2;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = s2[e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < S::NS; ++c)
+            if (!no_step<T, HD>(c, p.D)) {
+                s = mma_step<T>(TK::row(tk, rb, 0, 2 * c), q[c], s);
+                s2 = mma_step<T>(TK::row(tk, rb, 0, S::PH + 2 * c), q[c], s2);
+            }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = map ? s2[e] : s[e];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + 1 < n) {                                      // the next tile's keys after the scores, its values after the outputs
+            fetch_k(i + 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK) : "memory");      // this tile's values are there
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (kb + 32 > cut_from) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = kb + (e & 3) + 8 * (e >> 2) + 4 * lh < seen ? s[e] : -INFINITY;
+        }
+        Probs<T> pr, rest;
+        float sum;
+        auto weights = [&] {                                  // sum: this lane half's keys; the halves meet at the end
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -ref));
+                sum += w;
+                pr.set(e, w);
+                if constexpr (REST) rest.set(e, w - (float)(__bf16)w);
+            }
+        };
+        weights();
+        const bool again = mx == -INFINITY || sum > 1024.f;
+        if (__builtin_amdgcn_ballot_w64(again) != 0) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(s[e], s[e + 1]), top);
+            top = half_max(top) * p.c;
+            const bool move = top > mx;
+            const float a = move ? __builtin_amdgcn_exp2f(mx - top) : 1.f;
+            mx = move ? top : mx;
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= a;
+            weights();
+        }
+        l += sum;
+        mma_cols<T, S::RBV>(tv, cb, 0, 0, dvn, pr, o);
+        if constexpr (REST) mma_cols<T, S::RBV>(tv, cb, 0, 0, dvn, rest, o);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + 1 < n) fetch_v(i + 1);
+    }
+    l = half_sum(l);
+
+    // join the waves: a common maximum, then the outputs added in wave order, each element by one thread
+    if (lh == 0) {
+        ml[wave][l31][0] = mx;
+        ml[wave][l31][1] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][l31][0]);
+    const float f = __builtin_amdgcn_exp2f(mx - (top == -INFINITY ? 0.f : top));
+#pragma unroll
+    for (int d = 0; d < S::NDT; ++d)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+            *reinterpret_cast<f32x4*>(tk + l31 * (S::NDT * 128) + (((d * 8 + 2 * g4 + lh) ^ (l31 & 7)) << 4)) =
+                f32x4{o[d][4 * g4] * f, o[d][4 * g4 + 1] * f, o[d][4 * g4 + 2] * f, o[d][4 * g4 + 3] * f};
+    __syncthreads();
+    constexpr int PC = S::NDT * 8;                            // 16-byte pieces of a row and map
+    const int here = rows - r0 < 16 ? rows - r0 : 16;
+    for (int e = threadIdx.x; e < here * PC; e += NW * 64) {
+        const int row = e / PC, pc = e - row * PC, dd = pc * 4;
+        if (dd >= dvn) continue;
+        f32x4 out[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, st;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const int col = 16 * m + row;
+            float tp = -INFINITY, sum = 0.f;
+            for (int w = 0; w < NW; ++w) tp = fmaxf(tp, ml[w][col][0]);
+            for (int w = 0; w < NW; ++w) {
+                sum += ml[w][col][1] * __builtin_amdgcn_exp2f(ml[w][col][0] - (tp == -INFINITY ? 0.f : tp));
+                out[m] += *reinterpret_cast<const f32x4*>(stages + w * STAGE + col * (S::NDT * 128) + ((pc ^ (col & 7)) << 4));
+            }
+            st[2 * m] = tp;
+            st[2 * m + 1] = sum;
+        }
+        const bool lead = dd == 0 && vb == 0;
+        if (p.splits > 1) {
+            float* at = p.part + ((int64_t)sp * p.B * p.Hk * rows + (int64_t)bh * rows + r0 + row) * (2 * p.Dv + 4);
+            *reinterpret_cast<f32x4*>(at + dv0 + dd) = out[0];
+            *reinterpret_cast<f32x4*>(at + p.Dv + dv0 + dd) = out[1];
+            if (lead) *reinterpret_cast<f32x4*>(at + 2 * p.Dv) = st;
+            continue;
+        }
+        const int tt = (r0 + row) / p.g, h = r0 + row - tt * p.g;
+        diff_store<T>(p, ((int64_t)b * p.Tq + tt) * p.H + hk * p.g + h, dv0 + dd, out, st, lam_s[h], lead);
+    }
+}
+
+// Joins the splits of a row: a group of G lanes, 4 channels a lane.  The lanes share the reads that come before the outputs (the
+// lambda vectors, the splits' statistics), which by one lane each were the launch's whole time; from 8 splits on all groups of the
+// workgroup share a row (1 token, 32768 keys, 64 splits: 45 us of the call's 64 before).
 template <typename T>
-__global__ void __launch_bounds__(256) diff_join_kernel(const DiffArgs p) {
-    const int tpr = p.Dv / 4, rows = p.Tq * p.g;
-    const int64_t all = (int64_t)p.B * p.Hk * rows, row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / tpr;
-    const int dd = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) - row * tpr) * 4;
-    if (row >= all) return;
+__global__ void __launch_bounds__(256) diff_join_kernel(const DiffArgs p, int G, int groups) {
+    __shared__ float part[256][10];
+    const int rows = p.Tq * p.g, lane = threadIdx.x & (G - 1), dd = lane * 4, group = groups > 1 ? threadIdx.x / G : 0;
+    const int64_t all = (int64_t)p.B * p.Hk * rows, row = groups > 1 ? blockIdx.x : ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
+    if (row >= all) return;                                   // whole groups; whole workgroups where they share
     const int bh = (int)(row / rows), r = (int)(row - (int64_t)bh * rows), b = bh / p.Hk, hk = bh - b * p.Hk;
     const int t = r / p.g, head = hk * p.g + (r - t * p.g);
     const int LD = 2 * p.Dv + 4;
     const float* at = p.part + row * LD;
     const int64_t step = all * LD;
-    float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
+    float e1 = 0.f, e2 = 0.f, top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    {
+        const T* v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = static_cast<const T*>(p.lam_vec[i]) + head * p.lam_sh;
+        for (int d = lane; d < p.D; d += G) {
+            e1 = fmaf((float)v[0][d], (float)v[1][d], e1);
+            e2 = fmaf((float)v[2][d], (float)v[3][d], e2);
+        }
+    }
+    for (int s = lane; s < p.splits; s += G) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(at + s * step + 2 * p.Dv);
         top[0] = fmaxf(top[0], v[0]);
         top[1] = fmaxf(top[1], v[2]);
     }
+    for (int o = 1; o < G; o <<= 1) {
+        e1 += __shfl_xor(e1, o, 64);
+        e2 += __shfl_xor(e2, o, 64);
+        top[0] = fmaxf(top[0], __shfl_xor(top[0], o, 64));
+        top[1] = fmaxf(top[1], __shfl_xor(top[1], o, 64));
+    }
     f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int s = 0; s < p.splits; ++s) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(at + s * step + 2 * p.Dv);
+    if (dd < p.Dv) {
+#pragma unroll 4
+        for (int s = group; s < p.splits; s += groups) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(at + s * step + 2 * p.Dv);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const float f = __builtin_amdgcn_exp2f(v[2 * m] - (top[m] == -INFINITY ? 0.f : top[m]));
+                l[m] += v[2 * m + 1] * f;
+                o[m] += *reinterpret_cast<const f32x4*>(at + s * step + m * p.Dv + dd) * f;
+            }
+        }
+    }
+    if (groups > 1) {                                         // in group order
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const float f = __builtin_amdgcn_exp2f(v[2 * m] - (top[m] == -INFINITY ? 0.f : top[m]));
-            l[m] += v[2 * m + 1] * f;
-            o[m] += *reinterpret_cast<const f32x4*>(at + s * step + m * p.Dv + dd) * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[threadIdx.x][5 * m + e] = o[m][e];
+            part[threadIdx.x][5 * m + 4] = l[m];
         }
+        __syncthreads();
+        if (group) return;
+        for (int g = 1; g < groups; ++g)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[m][e] += part[g * G + lane][5 * m + e];
+                l[m] += part[g * G + lane][5 * m + 4];
+            }
     }
-    const T* v[4];
-    float e1 = 0.f, e2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = static_cast<const T*>(p.lam_vec[i]) + head * p.lam_sh;
-    for (int d = 0; d < p.D; d += 8) {
-        float x[4][8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_vec<T, 8>(v[i] + d, x[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            e1 = fmaf(x[0][e], x[1][e], e1);
-            e2 = fmaf(x[2][e], x[3][e], e2);
-        }
-    }
+    if (dd >= p.Dv) return;
     const f32x4 st = {top[0], l[0], top[1], l[1]};
     diff_store<T>(p, ((int64_t)b * p.Tq + t) * p.H + head, dd, o, st, expf(e1) - expf(e2) + p.lam_init, dd == 0);
 }
@@ -472,16 +577,18 @@ int diff_parts(int64_t units, int slots, int64_t length, int64_t grain, double p
     return best;
 }
 
-// Few rows: ~256 workgroups, one for each CU, no split under 256 keys (the case above: 51 us; 512 even out ragged lengths, but a
-// second start and join cost more: 58 us, 1024: 74).  Many: a workgroup's 32 keys take its CU ~30 HD cycles, fp32 ~190 HD.
+// Few rows: ~256 workgroups, one for each CU (the case above: 50 us; 512 even out ragged lengths, but a second start and join cost
+// more: 58 us, 1024: 74), no split under two tiles for each wave (4 x 8 heads, 2048 keys: 18 us for 20 with one).  Many: a workgroup's 32 keys take its CU ~30 HD cycles, fp32 ~190 HD.
 static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int es, int causal) {
     const int g = H / Hk, rows = Tq * g, hd = diff_head_dim(D, Dv);
     DiffPlan pl{rows <= 32, 1, Tk};
-    const int64_t units = (int64_t)B * Hk * (pl.few ? 1 : (rows + 127) / 128) * (hd == 128 ? (Dv + 127) / 128 : 1);
+    const int64_t units = (int64_t)B * Hk * (pl.few ? (rows + 15) / 16 : (rows + 127) / 128) * (hd == 128 ? (Dv + 127) / 128 : 1);
     if (pl.few) {
-        int64_t n = 256 / units, most = Tk > 255 * 64 ? 64 : (Tk + 255) / 256;
-        n = n < 1 ? 1 : (n < most ? n : most);
-        const int64_t chunk = ((Tk + n - 1) / n + 127) / 128 * 128;
+        const int tile = 32 * (2 * hd + (hd == 128 ? 128 : 2 * hd)) * es, grain = 32 * (tile <= 16384 ? 8 : (tile <= 32768 ? 4 : 2));      // a tile for each wave
+        int64_t n = 256 / units, most = (Tk + 2 * grain - 1) / (2 * grain);
+        n = n < most ? n : most;
+        n = n < 1 ? 1 : (n < 64 ? n : 64);
+        const int64_t chunk = ((Tk + n - 1) / n + grain - 1) / grain * grain;
         pl.chunk = (int)chunk;
         pl.splits = (int)((Tk + chunk - 1) / chunk);
     } else {
@@ -493,16 +600,19 @@ static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, i
     return pl;
 }
 
-template <typename T, int HD, bool FEW>
-static int launch_diff(const char* fn, const DiffArgs& a, hipStream_t st) {
-    const int rows = a.Tq * a.g, per = FEW ? 32 : 128;
+template <typename T, int HD>
+static int launch_diff(const char* fn, const DiffArgs& a, bool few, hipStream_t st) {
+    const int rows = a.Tq * a.g, per = few ? 16 : 128;
     const int vblocks = (a.Dv + DiffShape<T, HD>::DV - 1) / DiffShape<T, HD>::DV;
     const int64_t blocks = (int64_t)a.B * a.Hk * ((rows + per - 1) / per) * a.splits * vblocks;
     NDB_REQUIRE(blocks <= (1 << 24), fn, "too many workgroups for one launch");
-    hipLaunchKernelGGL((diff_attn_kernel<T, HD, FEW>), dim3((unsigned)blocks), dim3(diff_threads<T, HD, FEW>()), 0, st, a);
+    if (few) hipLaunchKernelGGL((diff_few_kernel<T, HD>), dim3((unsigned)blocks), dim3(64 * DiffShape<T, HD>::NW_FEW), 0, st, a);
+    else hipLaunchKernelGGL((diff_attn_kernel<T, HD>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     if (a.splits > 1) {
-        const int64_t threads = (int64_t)a.B * a.Hk * rows * (a.Dv / 4);
-        hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+        const int G = a.Dv <= 64 ? 16 : (a.Dv <= 128 ? 32 : 64);
+        const int64_t all = (int64_t)a.B * a.Hk * rows;
+        const int groups = a.splits >= 8 && all <= 16384 ? 256 / G : 1;
+        hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)(groups > 1 ? all : (all * G + 255) / 256)), dim3(256), 0, st, a, G, groups);
     }
     return check_launch(fn);
 }
@@ -510,9 +620,9 @@ static int launch_diff(const char* fn, const DiffArgs& a, hipStream_t st) {
 template <typename T>
 static int dispatch_diff(const char* fn, const DiffArgs& a, bool few, hipStream_t st) {
     switch (diff_head_dim(a.D, a.Dv)) {
-        case 32: return few ? launch_diff<T, 32, true>(fn, a, st) : launch_diff<T, 32, false>(fn, a, st);
-        case 64: return few ? launch_diff<T, 64, true>(fn, a, st) : launch_diff<T, 64, false>(fn, a, st);
-        default: return few ? launch_diff<T, 128, true>(fn, a, st) : launch_diff<T, 128, false>(fn, a, st);
+        case 32: return launch_diff<T, 32>(fn, a, few, st);
+        case 64: return launch_diff<T, 64>(fn, a, few, st);
+        default: return launch_diff<T, 128>(fn, a, few, st);
     }
 }
 

@@ -316,6 +316,7 @@ def test_feed_forward_of_more_than_2_32_bytes():
     (2, 1, 33, 64, 1, 128, 256, False), (1, 3, 65, 64, 1, 8, 8, True), (1, 32, 32, 1, 1, 64, 128, True), (1, 33, 257, 1, 1, 64, 128, True),
     (5, 1, 255, 3, 3, 32, 64, False), (5, 1, 256, 3, 3, 32, 64, False), (2, 1, 513, 3, 3, 32, 256, False), (1, 1, 20000, 2, 1, 16, 24, False),
     (1, 8, 1000, 8, 2, 128, 8, True), (40, 1, 300, 8, 8, 40, 72, False),
+    (1, 1, 40000, 3, 1, 64, 120, False), (1, 17, 5000, 1, 1, 32, 64, True), (2, 16, 2049, 2, 1, 128, 256, True),
 ])
 def test_differential_attention_sizes(B, Tq, Tk, H, Hk, D, Dv, causal, dtype):
     q, k, v = rnd(B, Tq, H, 2 * D, seed=1, dtype=dtype), rnd(B, Tk, Hk, 2 * D, seed=2, dtype=dtype), rnd(B, Tk, Hk, Dv, seed=3, dtype=dtype)
@@ -349,7 +350,7 @@ def test_differential_attention_scores_of_every_size():
 
 
 def test_differential_attention_bad_numbers_stay_in_their_row():
-    """A NaN or infinite query spoils its own row; a NaN value behind the causal edge of a row leaves that row alone."""
+    """A NaN or infinite query spoils its own row, NaN keys and values past a sequence's length none."""
     for dtype in (BF, F32):
         q, k, v = (rnd(1, 80, 1, 64, seed=i, dtype=dtype) for i in range(3))
         lams = [rnd(32, seed=4 + i, dtype=dtype, scale=0.2) for i in range(4)]
@@ -379,6 +380,20 @@ def test_feed_forward_of_few_rows(M, C, F, dtype):
     wide = torch.zeros(M, C + 24, device=DEV, dtype=dtype)       # rows of a wider tensor, no bias, no residual
     wide[:, 8:8 + C] = x
     assert torch.equal(block.gated_feed_forward(wide[:, 8:8 + C], w_in, w_out), block.gated_feed_forward(x, w_in, w_out))
+
+
+def test_differential_attention_infinite_key_of_one_map():
+    """A key that one map gives a score of -inf has no weight there and its ordinary one in the other map, alone and among many queries."""
+    D, Tk = 32, 70
+    for dtype in (BF, F32):
+        for Tq in (1, 40):
+            q, k, v = rnd(1, Tq, 2, 2 * D, seed=1, dtype=dtype), rnd(1, Tk, 2, 2 * D, seed=2, dtype=dtype), rnd(1, Tk, 2, 2 * D, seed=3, dtype=dtype)
+            q[..., 0], q[..., D] = 1, 1
+            k[0, 33, :, D], k[0, 5, :, 0] = -math.inf, -math.inf
+            lams = [rnd(D, seed=4 + i, dtype=dtype, scale=0.2) for i in range(4)]
+            o = block.differential_attention(q, k, v, *lams)
+            (ref, err), _ = diff_ref(*(t.double() for t in (q, k, v)), [t.double() for t in lams], 0.8, D ** -0.5, (Tk,), False, half_ulp(BF) if dtype == BF else 0.0)
+            assert torch.isfinite(ref).all() and within(o, ref, err, dtype)
 
 
 def test_feed_forward_bad_numbers_stay_in_their_row():
