@@ -3,14 +3,14 @@
 //   dV = (P1 - lam P2)^T dO     dS1 = P1 (dP - D1)     dS2 = -lam P2 (dP - D2)
 //   dq_i = s dS_i k_i           dk_i = s dS_i^T q_i    dlam = -sum P2 dP, which scales the gradients of the four vectors
 //
-// Three launches without atomics: D1 / D2; keys (a wave owns 32 keys, the rows of all query heads pass by: dk, dv and its share
-// of dlam); queries (a wave owns 32 rows, the keys pass by: dq).  Both rebuild the scores: 28 D T^2 operations for Dv = 2 D in all
+// Two launches without atomics: queries (a wave owns 32 rows, the keys pass by: D1, D2 and dq), then keys (a wave owns 32 keys, the
+// rows of all query heads pass by: dk, dv and its share of dlam), and a small one for the vectors.  Both rebuild the scores: 28 D T^2 operations for Dv = 2 D in all
 // where 20 would do with the maps kept, but nothing of T x T is stored.  Scores and dP come out of the matrix unit in the layout
 // in which dS is the next product's operand; the transposed operands are column reads of the same row-major tiles.
 // dlam is summed from fp32 P2 and dP, not from the rounded O2: it is one number and may cancel.  Rounding to bf16 besides the
 // outputs: P1 - lam P2, dS1, dS2 as operands, O1 and O2.  A sequence of one key has constant maps: dq and dk are made exactly zero.
 //
-// Measured, bf16, 8 x 2048^2 x 8 heads of 64 + 128, causal: D1 / D2 16 us, keys 250 us, queries 155 us (0.48 and 0.52 PFLOP/s of
+// Measured, bf16, 8 x 2048^2 x 8 heads of 64 + 128, causal: keys 250 us, queries 155 us (0.48 and 0.52 PFLOP/s of
 // matrix operations); what bounds them is what bounds the forward pass, with two exponentials and ~12 vector operations a score.
 #include "blk_diff_attn.h"
 
@@ -27,7 +27,6 @@ struct DiffBwdArgs {
     const float* lse;             // [2][B, Tq, H]
     float* dots;                  // [2][B, Tq, H]: D1, D2
     float* dlam_part;             // [B * Hk][key blocks][row splits][waves][g]
-    float* dlam;                  // [H]
     void *dq, *dk, *dv;           // contiguous
     void* dvec[4];
     int key_blocks, waves;        // of the key kernel: waves * 32 keys a workgroup
@@ -36,36 +35,20 @@ struct DiffBwdArgs {
     float *part_kv, *part_q;
 };
 
-// D1, D2 of a row: 16 lanes, 8 channels at a time
+// d += x . y over 16 bytes
 template <typename T>
-__global__ void __launch_bounds__(256) diff_dots_kernel(const DiffBwdArgs p) {
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, all = (int64_t)p.f.B * p.f.Tq * p.f.H;
-    if (row >= all) return;
-    const int lane = threadIdx.x & 15;
-    const int h = (int)(row % p.f.H);
-    const int64_t bt = row / p.f.H;
-    const int b = (int)(bt / p.f.Tq), t = (int)(bt - (int64_t)b * p.f.Tq);
-    const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.sb + t * p.dout.st + h * p.dout.sh;
-    float d1 = 0.f, d2 = 0.f;
-    for (int d = lane * 8; d < p.f.Dv; d += 128) {
-        float x[8], y[8], z[8];
-        load_vec<T, 8>(g + d, x);
-        load_vec<T, 8>(static_cast<const T*>(p.o1) + row * p.f.Dv + d, y);
-        load_vec<T, 8>(static_cast<const T*>(p.o2) + row * p.f.Dv + d, z);
+__device__ __forceinline__ void dot16(u32x4 x, u32x4 y, float& d) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            d1 = fmaf(x[e], y[e], d1);
-            d2 = fmaf(x[e], z[e], d2);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            union { unsigned u; bf16x2 h; } a, b;
+            a.u = x[i], b.u = y[i];
+            d = __builtin_amdgcn_fdot2_f32_bf16(a.h, b.h, d, false);
+        } else {
+            union { unsigned u; float f; } a, b;
+            a.u = x[i], b.u = y[i];
+            d = fmaf(a.f, b.f, d);
         }
-    }
-#pragma unroll
-    for (int o = 8; o; o >>= 1) {
-        d1 += __shfl_xor(d1, o, 64);
-        d2 += __shfl_xor(d2, o, 64);
-    }
-    if (lane == 0) {
-        p.dots[row] = d1;
-        p.dots[all + row] = d2;
     }
 }
 
@@ -355,7 +338,26 @@ __global__ void __launch_bounds__(256, (HD * (int)sizeof(T) >= 256 ? 1 : 2)) dif
         }
     }
     const int64_t orow = ((int64_t)b * f.Tq + t) * f.H + head, rows_all = (int64_t)f.B * f.Tq * f.H;
-    const float l1 = p.lse[orow], l2 = p.lse[rows_all + orow], c1 = p.dots[orow], c2 = p.dots[rows_all + orow];
+    const float l1 = p.lse[orow], l2 = p.lse[rows_all + orow];
+    float c1 = 0.f, c2 = 0.f;                                 // D1, D2: kept for the key kernel
+    {
+        const char* p1 = reinterpret_cast<const char*>(static_cast<const T*>(p.o1) + orow * f.Dv);
+        const char* p2 = reinterpret_cast<const char*>(static_cast<const T*>(p.o2) + orow * f.Dv);
+#pragma unroll
+        for (int c = 0; c < S::NSV; ++c) {
+            const int by = (2 * c + lh) * 16;
+            if (by < f.Dv * S::ES) {
+                dot16<T>(go[c], *reinterpret_cast<const u32x4*>(p1 + by), c1);
+                dot16<T>(go[c], *reinterpret_cast<const u32x4*>(p2 + by), c2);
+            }
+        }
+        c1 = half_sum(c1);
+        c2 = half_sum(c2);
+        if (ks == 0 && lh == 0 && r0 + l31 < rows) {
+            p.dots[orow] = c1;
+            p.dots[rows_all + orow] = c2;
+        }
+    }
     __syncthreads();
     const float nlam = -lam_s[hg];
     f32x16 dq[2][HD / 32];
@@ -468,36 +470,35 @@ __global__ void __launch_bounds__(256) diff_bwd_join_kernel(const DiffBwdArgs p)
     }
 }
 
-// dlam[h]: the partials of one head in a fixed order
-__global__ void __launch_bounds__(256) diff_dlam_kernel(const DiffBwdArgs p) {
-    __shared__ float red[256];
-    const int head = blockIdx.x, hk = head / p.f.g, hg = head - hk * p.f.g, per = p.key_blocks * p.row_splits * p.waves;
-    float t = 0.f;
-    for (int i = threadIdx.x; i < p.f.B * per; i += 256) {
-        const int b = i / per, j = i - b * per;
-        t += p.dlam_part[(((int64_t)b * p.f.Hk + hk) * per + j) * p.f.g + hg];
-    }
-    red[threadIdx.x] = t;
-    __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) p.dlam[head] = red[0];
-}
-
-// the four vectors' gradients: one wave per head, or one for all heads where they share the vectors
+// The four vectors' gradients from the partial dlam, summed in a fixed order: a workgroup per head, or one for all heads where they
+// share the vectors.
 template <typename T>
-__global__ void __launch_bounds__(64) diff_dvec_kernel(const DiffBwdArgs p) {
-    const int lane = threadIdx.x;
+__global__ void __launch_bounds__(1024) diff_dvec_kernel(const DiffBwdArgs p) {
+    __shared__ float red[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, per = p.key_blocks * p.row_splits * p.waves;
+    float t = 0.f;
+    if (p.f.lam_sh) {
+        const int hk = head / p.f.g, hg = head - hk * p.f.g;
+        for (int i = threadIdx.x; i < p.f.B * per; i += 1024) {
+            const int b = i / per, j = i - b * per;
+            t += p.dlam_part[(((int64_t)b * p.f.Hk + hk) * per + j) * p.f.g + hg];
+        }
+    } else {
+        const int64_t all = (int64_t)p.f.B * p.f.Hk * per * p.f.g;
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < all; i += 1024) t += p.dlam_part[i];
+    }
     float e1, e2;
-    diff_lambda<T>(p.f, p.f.lam_sh ? (int)blockIdx.x : 0, lane, e1, e2);
+    diff_lambda<T>(p.f, head, lane, e1, e2);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (lane == 0) red[wave] = t;
+    __syncthreads();
+    if (wave) return;
     float dlam = 0.f;
-    if (p.f.lam_sh)
-        dlam = p.dlam[blockIdx.x];
-    else
-        for (int h = 0; h < p.f.H; ++h) dlam += p.dlam[h];
-    const int64_t at = blockIdx.x * p.f.lam_sh;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) dlam += red[w];
+    const int64_t at = head * p.f.lam_sh;
     for (int d = lane; d < p.f.D; d += 64) {
         const T* v[4];
 #pragma unroll
@@ -517,8 +518,8 @@ static int launch_dkv(const char* fn, const DiffBwdArgs& a, hipStream_t st) {
 
 template <typename T, int HD>
 static int launch_diff_bwd(const char* fn, const DiffBwdArgs& a, hipStream_t st) {
-    const int64_t rows = (int64_t)a.f.B * a.f.Tq * a.f.H;
-    hipLaunchKernelGGL((diff_dots_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
+    const int tiles = (a.f.Tq * a.f.g + 127) / 128;
+    hipLaunchKernelGGL((diff_dq_kernel<T, HD>), dim3((unsigned)(a.f.B * a.f.Hk * tiles * a.key_splits)), dim3(256), 0, st, a);
     if constexpr (HD == 128) {
         if (int rc = launch_dkv<T, HD, 4, true, false>(fn, a, st)) return rc;
         if (int rc = launch_dkv<T, HD, 4, false, true>(fn, a, st)) return rc;
@@ -527,13 +528,9 @@ static int launch_diff_bwd(const char* fn, const DiffBwdArgs& a, hipStream_t st)
     } else {
         if (int rc = launch_dkv<T, HD, 4, true, true>(fn, a, st)) return rc;
     }
-    const int tiles = (a.f.Tq * a.f.g + 127) / 128;
-    hipLaunchKernelGGL((diff_dq_kernel<T, HD>), dim3((unsigned)(a.f.B * a.f.Hk * tiles * a.key_splits)), dim3(256), 0, st, a);
     if (a.row_splits > 1 || a.key_splits > 1) hipLaunchKernelGGL((diff_bwd_join_kernel<T>), dim3(1024), dim3(256), 0, st, a);
-    if (a.dvec[0] || a.dvec[1] || a.dvec[2] || a.dvec[3]) {
-        hipLaunchKernelGGL(diff_dlam_kernel, dim3((unsigned)a.f.H), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((diff_dvec_kernel<T>), dim3((unsigned)(a.f.lam_sh ? a.f.H : 1)), dim3(64), 0, st, a);
-    }
+    if (a.dvec[0] || a.dvec[1] || a.dvec[2] || a.dvec[3])
+        hipLaunchKernelGGL((diff_dvec_kernel<T>), dim3((unsigned)(a.f.lam_sh ? a.f.H : 1)), dim3(1024), 0, st, a);
     return check_launch(fn);
 }
 
@@ -559,7 +556,7 @@ static DiffBwdPlan diff_bwd_plan(int B, int Tq, int Tk, int H, int Hk, int D, in
     pl.key_splits = diff_parts(units * (((int64_t)Tq * g + 127) / 128), hd * es >= 256 ? 256 : 512, Tk, 64, (es == 4 ? 8.0 : 1.3) * hd, (double)rows * 2 * D * 4, causal, share);
     pl.chunk = (int)share;
     pl.dots = 2 * rows;
-    pl.dlam = ((units * pl.key_blocks * pl.row_splits * pl.waves * g + H) + 3) / 4 * 4;
+    pl.dlam = (units * pl.key_blocks * pl.row_splits * pl.waves * g + 3) / 4 * 4;
     pl.kv = pl.row_splits > 1 ? pl.row_splits * krows * (2 * D + Dv) : 0;
     pl.q = pl.key_splits > 1 ? pl.key_splits * rows * 2 * D : 0;
     pl.dots = (pl.dots + 3) / 4 * 4;
@@ -621,7 +618,6 @@ extern "C" int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, 
     p.dvec[0] = dlambda_q1, p.dvec[1] = dlambda_k1, p.dvec[2] = dlambda_q2, p.dvec[3] = dlambda_k2;
     p.dots = workspace;
     p.dlam_part = workspace + pl.dots;
-    p.dlam = p.dlam_part + (int64_t)B * Hk * pl.key_blocks * pl.row_splits * pl.waves * a.g;
     p.part_kv = workspace + pl.dots + pl.dlam;
     p.part_q = p.part_kv + pl.kv;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
