@@ -94,6 +94,19 @@ int nd_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
                      int C, int F, int act, int dtype, nd_stream_t stream);
 int64_t nd_gated_ffn_bwd_workspace_floats(int M, int C, int F, int dtype);
 
+/* ---- one array of arguments ------------------------------------------------------------------------------------------- */
+
+#define ND_CALL_QK_NORM_ROPE 0
+#define ND_CALL_QK_NORM_ROPE_BWD 1
+#define ND_CALL_DIFF_ATTENTION 2
+#define ND_CALL_DIFF_ATTENTION_BWD 3
+#define ND_CALL_GATED_FFN 4
+#define ND_CALL_GATED_FFN_BWD 5
+
+/* The call above with its arguments (all but the stream) as 8-byte words in their order: pointers and integers as they are, floats as
+ * doubles.  For callers through a foreign-function interface, whose cost is per argument. */
+int nd_block_packed(int call, const int64_t* words, int count, nd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

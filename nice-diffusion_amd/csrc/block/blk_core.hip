@@ -1,4 +1,4 @@
-// Bookkeeping of libnd_block.so: last-error string (thread-local), build id, and the ordered sum of partial rows.
+// Bookkeeping of libnd_block.so: last-error string (thread-local) and build id.
 #include "blk_common.h"
 
 namespace ndb {

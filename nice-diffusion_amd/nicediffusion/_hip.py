@@ -6,6 +6,7 @@ path raises.  PyTorch is used only for device memory, streams and graph capture.
 """
 import ctypes
 import os
+import struct
 
 _LIB = None
 _LIB_PATH = os.environ.get('ND_HIP_LIB') or os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libnd_hip.so')
@@ -160,7 +161,12 @@ BLOCK_SIGNATURES = {
     'nd_gated_ffn_workspace_floats': ([_i] * 4, _i64),
     'nd_gated_ffn_bwd': ([_vp, _i64, _vp, _i64] + [_vp] * 11 + [_i] * 5 + [_vp], _i),
     'nd_gated_ffn_bwd_workspace_floats': ([_i] * 4, _i64),
+    'nd_block_packed': ([_i, ctypes.c_char_p, _i, _vp], _i),
 }
+# calls that nd_block_packed takes, in the order of its ND_CALL_*: (index, packer of all arguments but the stream, their number)
+BLOCK_CALLS = {n: (k, struct.Struct(''.join('d' if a is _f else 'q' for a in BLOCK_SIGNATURES[n][0][:-1])), len(BLOCK_SIGNATURES[n][0]) - 1)
+               for k, n in enumerate(('nd_qk_norm_rope', 'nd_qk_norm_rope_bwd', 'nd_diff_attention', 'nd_diff_attention_bwd', 'nd_gated_ffn',
+                                      'nd_gated_ffn_bwd'))}
 _BLOCK = None
 _BLOCK_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libnd_block.so')
 

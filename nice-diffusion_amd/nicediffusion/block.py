@@ -76,15 +76,19 @@ def _stream(index):
 
 def _call(name, device, *args):
     """Launch ``name`` on the current stream of ``device`` (made the current device for the call)."""
-    fn = getattr(_hip.load_block(), name)
-    index = device.index
+    call, pack, n = _hip.BLOCK_CALLS[name]
+    fn, words, index = _hip.load_block().nd_block_packed, pack.pack(*args), device.index
     if torch.cuda.current_device() == index:
-        rc = fn(*args, _stream(index))
+        rc = fn(call, words, n, _stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _stream(index))
+            rc = fn(call, words, n, _stream(index))
     if rc:
         _hip.check_block(rc, name)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _aligned(t):
@@ -159,8 +163,8 @@ def _table_stride(t):
 def _launch_qk(q, k, qw, kw, cos, sin, eps, interleaved, qo, ko):
     B, T, Hq, D = q.shape
     R, tb = 0 if cos is None else 2 * cos.shape[-1], _table_stride(cos)
-    _call('nd_qk_norm_rope', q.device, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), _hip.ptr(qw), _hip.ptr(kw), _hip.ptr(cos),
-          _hip.ptr(sin), tb, qo.data_ptr(), *_strides(qo), ko.data_ptr(), *_strides(ko), B, T, Hq, k.shape[2], D, R, eps,
+    _call('nd_qk_norm_rope', q.device, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), _ptr(qw), _ptr(kw), _ptr(cos),
+          _ptr(sin), tb, qo.data_ptr(), *_strides(qo), ko.data_ptr(), *_strides(ko), B, T, Hq, k.shape[2], D, R, eps,
           _hip.ROPE_INTERLEAVED if interleaved else 0, _DT[q.dtype])
 
 
@@ -190,9 +194,9 @@ class _QkNormRope(torch.autograd.Function):
                 n = _hip.load_block().nd_qk_norm_rope_bwd_workspace_floats(B, T, Hq, Hk, D)
                 ws = torch.empty(n, dtype=torch.float32, device=q.device)
             R, tb = 0 if cos is None else 2 * cos.shape[-1], _table_stride(cos)
-            _call('nd_qk_norm_rope_bwd', q.device, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), _hip.ptr(qw), _hip.ptr(kw),
-                  _hip.ptr(cos), _hip.ptr(sin), tb, dqo.data_ptr(), *_strides(dqo), dko.data_ptr(), *_strides(dko), dq.data_ptr(),
-                  *_strides(dq), dk.data_ptr(), *_strides(dk), _hip.ptr(dqw), _hip.ptr(dkw), _hip.ptr(ws), B, T, Hq, Hk, D, R, ctx.eps,
+            _call('nd_qk_norm_rope_bwd', q.device, q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), _ptr(qw), _ptr(kw),
+                  _ptr(cos), _ptr(sin), tb, dqo.data_ptr(), *_strides(dqo), dko.data_ptr(), *_strides(dko), dq.data_ptr(),
+                  *_strides(dq), dk.data_ptr(), *_strides(dk), _ptr(dqw), _ptr(dkw), _ptr(ws), B, T, Hq, Hk, D, R, ctx.eps,
                   _hip.ROPE_INTERLEAVED if ctx.interleaved else 0, _DT[q.dtype])
         else:
             for g in (dqw, dkw):
@@ -278,7 +282,7 @@ def _diff_args(q, k, v, lams, lambda_init, lengths):
     per_head = lams[0].dim() == 2
     lq1, lk1, lq2, lk2 = lams
     return (q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), lq1.data_ptr(), lk1.data_ptr(), lq2.data_ptr(),
-            lk2.data_ptr(), lq1.shape[-1] if per_head else 0, lambda_init, _hip.ptr(lengths))
+            lk2.data_ptr(), lq1.shape[-1] if per_head else 0, lambda_init, _ptr(lengths))
 
 
 def _diff_sizes(q, k, v):
@@ -292,8 +296,8 @@ def _launch_diff(q, k, v, lams, lambda_init, scale, lengths, causal, keep):
     out = q.new_empty(B, Tq, H, Dv)
     o1, o2, lse = (torch.empty_like(out), torch.empty_like(out), _floats(2 * B * Tq * H, q.device)) if keep else (None,) * 3
     ws = _floats(_hip.load_block().nd_diff_attention_workspace_floats(*sizes, _DT[q.dtype]), q.device)
-    _call('nd_diff_attention', q.device, *_diff_args(q, k, v, lams, lambda_init, lengths), out.data_ptr(), _hip.ptr(o1), _hip.ptr(o2),
-          _hip.ptr(lse), _hip.ptr(ws), *sizes, scale, _hip.ATTN_CAUSAL if causal else 0, _DT[q.dtype])
+    _call('nd_diff_attention', q.device, *_diff_args(q, k, v, lams, lambda_init, lengths), out.data_ptr(), _ptr(o1), _ptr(o2),
+          _ptr(lse), _ptr(ws), *sizes, scale, _hip.ATTN_CAUSAL if causal else 0, _DT[q.dtype])
     return out, o1, o2, lse
 
 
@@ -318,7 +322,7 @@ class _DiffAttention(torch.autograd.Function):
         dl = [torch.empty_like(t) if n else None for t, n in zip(lams, ctx.needs_input_grad[3:7])]
         ws = _floats(_hip.load_block().nd_diff_attention_bwd_workspace_floats(*sizes, _DT[q.dtype]), q.device)
         _call('nd_diff_attention_bwd', q.device, *_diff_args(q, k, v, lams, ctx.lambda_init, lengths), o1.data_ptr(), o2.data_ptr(),
-              lse.data_ptr(), dout.data_ptr(), *_strides(dout), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *(_hip.ptr(t) for t in dl),
+              lse.data_ptr(), dout.data_ptr(), *_strides(dout), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *(_ptr(t) for t in dl),
               ws.data_ptr(), *sizes, ctx.scale, _hip.ATTN_CAUSAL if ctx.causal else 0, _DT[q.dtype])
         return (dq, dk, dv, *dl, None, None, None, None)
 
@@ -399,8 +403,8 @@ def _launch_ffn(x, w_in, b_in, w_out, b_out, res, act, keep, shape):
     y, h = x.new_empty(shape), x.new_empty(M, F)
     au = x.new_empty(M, 2 * F) if keep else None
     ws = _floats(_hip.load_block().nd_gated_ffn_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
-    _call('nd_gated_ffn', x.device, x.data_ptr(), _ld(x), w_in.data_ptr(), _hip.ptr(b_in), w_out.data_ptr(), _hip.ptr(b_out), _hip.ptr(res),
-          0 if res is None else _ld(res), y.data_ptr(), C, h.data_ptr(), _hip.ptr(au), _hip.ptr(ws), M, C, F, act, _DT[x.dtype])
+    _call('nd_gated_ffn', x.device, x.data_ptr(), _ld(x), w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out), _ptr(res),
+          0 if res is None else _ld(res), y.data_ptr(), C, h.data_ptr(), _ptr(au), _ptr(ws), M, C, F, act, _DT[x.dtype])
     return y, h, au
 
 
@@ -437,7 +441,7 @@ class _GatedFfn(torch.autograd.Function):
                 dau = torch.empty(M, 2 * F, **new) if any(need[:3]) else None
                 ws = _floats(_hip.load_block().nd_gated_ffn_bwd_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
                 _call('nd_gated_ffn_bwd', x.device, g.data_ptr(), _ld(g), x.data_ptr(), _ld(x), w_in.data_ptr(), w_out.data_ptr(), au.data_ptr(),
-                      h.data_ptr(), _hip.ptr(dx), _hip.ptr(dwi), _hip.ptr(dbi), _hip.ptr(dwo), _hip.ptr(dbo), _hip.ptr(dau), _hip.ptr(ws), M, C,
+                      h.data_ptr(), _ptr(dx), _ptr(dwi), _ptr(dbi), _ptr(dwo), _ptr(dbo), _ptr(dau), _ptr(ws), M, C,
                       F, ctx.act, _DT[x.dtype])
         else:
             for t in (dwi, dbi, dwo, dbo):

@@ -114,6 +114,25 @@ def test_c_backward_calls_refuse():
     assert lib.nd_diff_attention_bwd_workspace_floats(1, 0, 1, 2, 2, 32, 64, _hip.DT_BF16) < 0
 
 
+def test_packed_calls_are_the_plain_ones():
+    """Same refusals through nd_block_packed; a wrong count, an unknown call and an integer too large for its type are refused."""
+    lib = _hip.load_block()
+    plain = {'nd_qk_norm_rope': (qk_args(D=63), 'even'), 'nd_diff_attention': (diff_args(scale=0.0), 'scale'), 'nd_gated_ffn': (ffn_args(act=3), 'activation')}
+    for name, (args, what) in plain.items():
+        k, pack, n = _hip.BLOCK_CALLS[name]
+        words = pack.pack(*[0 if a is None else a for a in args[:-1]])
+        assert len(words) == 8 * n
+        assert lib.nd_block_packed(k, words, n, None) == -1 and re.search(what, lib.nd_block_last_error().decode())
+        assert lib.nd_block_packed(k, words, n - 1, None) == -1 and b'number' in lib.nd_block_last_error()
+    assert lib.nd_block_packed(17, words, n, None) == -1 and b'unknown' in lib.nd_block_last_error()
+    k, pack, n = _hip.BLOCK_CALLS['nd_gated_ffn']
+    words = pack.pack(*[0 if a is None else a for a in ffn_args(M=(1 << 32) + 5)[:-1]])
+    assert lib.nd_block_packed(k, words, n, None) == -1 and b'fit' in lib.nd_block_last_error()
+    header = open(os.path.join(ROOT, 'include', 'nd_block.h')).read()
+    for name, (k, _, _) in _hip.BLOCK_CALLS.items():
+        assert re.search(r'#define ND_CALL_{} {}\b'.format(name[3:].upper(), k), header), name
+
+
 def test_workspaces_are_as_large_as_the_splits_need():
     """Divided keys and contractions: one fp32 partial row per split; nothing where the chip is full without."""
     lib = _hip.load_block()
