@@ -379,12 +379,13 @@ struct Plan {
     int splits, k_tiles;
 };
 
-// Time of a product in cycles of a CU (2.2 GHz), from measured ones.  A workgroup's stage (128 bytes of k): bf16 3700 / 1120 / 500
-// at ti 4 / 2 / 1 (LDS and L2 traffic per operation: 275 GFLOP, 16384 x 1024 x 8192, took 230 / 265 / 484 us), fp32 the matrix
-// units' 1024 ti^2.  4 / ti workgroups share a CU; a stage takes ~1200 to arrive.  What the epilogue moves (`moved`, bytes) goes at
-// ~5 TB/s, worse where one workgroup has the CU to itself and nothing overlaps it: the gate's backward product at
-// 16384 x 4096 x 1024 takes 266 / 214 / 272 us, its forward one 283 / 305 / 418.
-static Plan plan_gemm(int64_t M, int64_t N, int64_t K, int es, bool gated, bool may_split, double moved) {
+// Time of a product in cycles of a CU (2.2 GHz), the constants fitted to 180 products of 20 feed-forward shapes, each timed with every
+// tile and several divisions (the choices then cost 1.2 % over the best ones; 300 x 136 to 65536 x 2048).  A workgroup's stage (128
+// bytes of k): bf16 3200 / 1120 / 380 at ti 4 / 2 / 1 (LDS and L2 traffic per operation: 275 GFLOP, 16384 x 1024 x 8192, took
+// 230 / 265 / 484 us), fp32 the matrix units' 1024 ti^2, ti 1 a fifth more.  4 / ti workgroups share a CU; a stage takes ~850 to
+// arrive.  What the epilogue moves (`moved`, bytes) goes at ~5 TB/s, worse where one workgroup has the CU to itself and nothing
+// overlaps it (so does gelu's arithmetic: 65536 x 384 x 1024 forward 228 us with ti 4, 210 with 2): the gate's backward product at 16384 x 4096 x 1024 takes 266 / 214 / 272 us, its forward one 283 / 305 / 418.
+static Plan plan_gemm(int64_t M, int64_t N, int64_t K, int es, bool gated, bool gelu, bool may_split, double moved) {
     const int kt = 128 / es;
     const int64_t stages = (K + kt - 1) / kt;
     Plan best{};
@@ -392,17 +393,18 @@ static Plan plan_gemm(int64_t M, int64_t N, int64_t K, int es, bool gated, bool 
     for (int ti = 4; ti; ti /= 2) {
         const int tile = 64 * ti;
         const int64_t tiles = ((M + tile - 1) / tile) * ((N + (gated ? tile / 2 : tile) - 1) / (gated ? tile / 2 : tile));
-        const double stage = es == 4 ? (ti == 1 ? 1060.0 : 1024.0 * ti * ti) : (ti == 4 ? 3700.0 : (ti == 2 ? 1120.0 : 500.0));
-        const double epilogue = moved / 2340.0 * (ti == 4 ? 1.2 : (ti == 2 ? 0.85 : 0.6));
+        const double stage = es == 4 ? (ti == 1 ? 1220.0 : 1024.0 * ti * ti) : (ti == 4 ? 3200.0 : (ti == 2 ? 1120.0 : 380.0));
+        const double epilogue = moved / 2340.0 * (ti == 4 ? 1.2 : (ti == 2 ? 0.8 : 0.7));
         for (int want = 1; want <= (may_split ? 64 : 1); want *= 2) {
             const int64_t per = (stages + want - 1) / want;
             const int64_t splits = (stages + per - 1) / per;
             if (want > 1 && (per < 4 || splits * M * N > (1LL << 28))) break;
             const int64_t each = (tiles * splits + 255) / 256, rounds = (each + 4 / ti - 1) / (4 / ti);      // workgroups a CU
-            const double work = (double)each * per * stage, wait = (double)rounds * per * 1200.0;
-            double t = (work > wait ? work : wait) + (double)rounds * (ti == 4 ? 9000.0 : 2000.0 + 500.0 * ti) + epilogue;
-            // the join moves splits + 1 fp32 copies at ~2 KiB a cycle over the chip, and is a launch of its own
-            if (splits > 1) t += 5000.0 + (double)(splits + 1) * M * N * 4 / 2048.0;
+            const double work = (double)each * per * stage, wait = (double)rounds * per * 850.0;
+            double t = (work > wait ? work : wait) + (double)rounds * (ti == 4 ? 8200.0 : (ti == 2 ? 4600.0 : 2600.0)) + epilogue;
+            if (gelu) t += (double)each * (ti == 4 ? 14000.0 : (ti == 2 ? 600.0 : 150.0));
+            // the join moves splits + 1 fp32 copies at ~1.7 KiB a cycle over the chip, and is a launch of its own
+            if (splits > 1) t += 11000.0 + (double)(splits + 1) * M * N * 4 / 1700.0;
             if (t < best_t) {
                 best_t = t;
                 best = {ti, (int)splits, (int)per};
@@ -441,7 +443,7 @@ static int run_gemm(const char* fn, const GemmSide<T>& x, const GemmSide<T>& w, 
 // a product whose contraction may be split: straight to the output, or partials and their join
 template <typename T, bool XK, bool WK>
 static int run_gemm_out(const char* fn, const GemmSide<T>& x, const GemmSide<T>& w, int K, float* ws, const EpiOut<T>& epi, hipStream_t st) {
-    const Plan pl = plan_gemm(x.n, w.n, K, sizeof(T), false, true, (double)x.n * w.n * sizeof(T));
+    const Plan pl = plan_gemm(x.n, w.n, K, sizeof(T), false, false, true, (double)x.n * w.n * sizeof(T));
     if (pl.splits == 1) return run_gemm<T, XK, WK>(fn, x, w, K, pl, 0, epi, st);
     NDB_REQUIRE(ws, fn, "workspace missing");
     const EpiPart part{ws, w.n, (int64_t)x.n * w.n};
@@ -453,7 +455,7 @@ static int run_gemm_out(const char* fn, const GemmSide<T>& x, const GemmSide<T>&
 }
 
 static int64_t split_floats(int64_t M, int64_t N, int64_t K, int es) {
-    const Plan pl = plan_gemm(M, N, K, es, false, true, (double)M * N * es);
+    const Plan pl = plan_gemm(M, N, K, es, false, false, true, (double)M * N * es);
     return pl.splits > 1 ? pl.splits * M * N : 0;
 }
 
@@ -489,7 +491,7 @@ static int ffn_forward(const char* fn, const Ffn<T>& a, hipStream_t st) {
         if (int rc = run_few<T, 8>(fn, a.x, a.ldx, a.w_in, a.M, a.F, a.C, gate, st)) return rc;
         return run_few<T, 16>(fn, a.h, a.F, a.w_out, a.M, a.C, a.F, down, st);
     }
-    const Plan pl = plan_gemm(a.M, a.F, a.C, sizeof(T), true, false, (a.au ? 3.0 : 1.0) * a.M * a.F * sizeof(T));
+    const Plan pl = plan_gemm(a.M, a.F, a.C, sizeof(T), true, ACT != ND_ACT_SILU, false, (a.au ? 3.0 : 1.0) * a.M * a.F * sizeof(T));
     if (int rc = run_gemm<T, true, true>(fn, GemmSide<T>{a.x, a.ldx, a.M}, GemmSide<T>{a.w_in, a.C, 2 * a.F}, a.C, pl, a.F, gate, st))
         return rc;
     return run_gemm_out<T, true, true>(fn, GemmSide<T>{a.h, a.F, a.M}, GemmSide<T>{a.w_out, a.F, a.C}, a.F, a.ws, down, st);
@@ -508,7 +510,7 @@ template <typename T, int ACT>
 static int ffn_backward(const char* fn, const FfnBwd<T>& a, hipStream_t st) {
     const int M = a.M, C = a.C, F = a.F;
     if (a.dau) {
-        const Plan pl = plan_gemm(M, F, C, sizeof(T), false, false, 4.0 * M * F * sizeof(T));
+        const Plan pl = plan_gemm(M, F, C, sizeof(T), false, ACT != ND_ACT_SILU, false, 4.0 * M * F * sizeof(T));
         if (int rc = run_gemm<T, true, false>(fn, GemmSide<T>{a.dy, a.lddy, M}, GemmSide<T>{a.w_out, F, F}, C, pl, 0,
                                               EpiGateBwd<T, ACT>{a.au, a.dau, F}, st))
             return rc;
