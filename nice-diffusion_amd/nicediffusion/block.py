@@ -224,6 +224,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
         raise ValueError('head dim must be even and at most 512, got {}'.format(D))
     if Hq == 0 or k.shape[2] == 0:
         raise ValueError('q and k need at least one head')
+    if not 0 <= eps < float('inf'):
+        raise ValueError('eps must be finite and not negative, got {}'.format(eps))
     if q_weight is not None:
         _shape(q_weight, 'q_weight', D)
         q_weight = _aligned(q_weight)

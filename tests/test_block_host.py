@@ -156,6 +156,7 @@ T4 = (2, 5, 3, 16)
     ((z(5, 3, 16), z(*T4)), {}, ValueError, 'q has shape'), ((z(*T4), z(5, 3, 16)), {}, ValueError, 'k has shape'),
     ((z(*T4), z(2, 6, 3, 16)), {}, ValueError, 'k has shape'), ((z(2, 5, 3, 15), z(2, 5, 3, 15)), {}, ValueError, 'even'),
     ((z(2, 5, 3, 514), z(2, 5, 3, 514)), {}, ValueError, '512'), ((z(2, 5, 0, 16), z(*T4)), {}, ValueError, 'head'),
+    ((z(*T4), z(*T4)), {'eps': -1e-6}, ValueError, 'eps'), ((z(*T4), z(*T4)), {'eps': float('nan')}, ValueError, 'eps'),
     ((z(*T4), z(*T4), z(8)), {}, ValueError, 'q_weight'), ((z(*T4), z(*T4), None, z(1, 16)), {}, ValueError, 'k_weight'),
     ((z(*T4), z(*T4), None, None, z(5, 8)), {}, ValueError, 'together'), ((z(*T4), z(*T4), None, None, z(5, 8), z(5, 7)), {}, ValueError, 'sin'),
     ((z(*T4), z(*T4), None, None, z(4, 8), z(4, 8)), {}, ValueError, 'cos has shape'), ((z(*T4), z(*T4), None, None, z(5, 9), z(5, 9)), {}, ValueError, '18 channels'),
