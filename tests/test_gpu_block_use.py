@@ -312,6 +312,32 @@ def test_feed_forward_of_more_than_2_32_bytes():
 
 # ----------------------------------------------------------------------------------------------------- ends of the ranges
 @pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('B,T,Hq,Hk,D,R', [(1, 1, 1, 1, 64, 64), (3, 5, 3, 2, 64, 64), (1, 1, 1, 2, 32, 32), (2, 37, 5, 2, 32, 0), (1, 3, 1, 1, 16, 16),
+                                           (5, 1, 2, 1, 64, 0), (1, 1031, 1, 1, 64, 64), (1, 67, 3, 1, 8, 8)])
+def test_norm_and_rotation_of_short_rows(B, T, Hq, Hk, D, R, dtype):
+    """Rows of at most 256 bytes, several to a wave: odd numbers of rows, waves that span queries and keys, eps = 0, in place."""
+    q, k = rnd(B, T, Hq, D, seed=1, dtype=dtype), rnd(B, T, Hk, D, seed=2, dtype=dtype)
+    w = [rnd(D, seed=3 + i, dtype=dtype, scale=0.2, mean=1.0) for i in range(2)]
+    cos, sin = block.rotary_table(torch.arange(T, device=DEV), R) if R else (None, None)
+    leaves = [t.clone().requires_grad_() for t in (q, k, *w)]
+    wide = [t.double().requires_grad_() for t in (q, k, *w)]
+    outs = block.qk_norm_rope(*leaves, cos, sin, eps=0.0)
+    refs = [qk_ref(wide[i], wide[2 + i], cos, sin, 0.0, False) for i in range(2)]
+    tol = half_ulp(dtype) + fp32_tol(D) + 8 * half_ulp(F32)
+    for o, r in zip(outs, refs):
+        assert rel(o, r) <= tol
+    douts = [rnd(*o.shape, seed=7 + i, dtype=dtype) for i, o in enumerate(outs)]
+    for i, (g, r) in enumerate(zip(torch.autograd.grad(outs, leaves, douts), torch.autograd.grad(refs, wide, [d.double() for d in douts]))):
+        n = D if i < 2 else B * T * (Hq, Hk)[i - 2]
+        assert rel(g, r) <= half_ulp(dtype) + 2 * fp32_tol(D) + fp32_tol(n) + 16 * half_ulp(F32), i
+    room = torch.full((B, T + 1, Hq + Hk + 1, D), 7.0, device=DEV, dtype=dtype)      # in place in wider rows: the rest stays
+    room[:, :T, :Hq], room[:, :T, Hq:Hq + Hk] = q, k
+    a, b = room[:, :T, :Hq], room[:, :T, Hq:Hq + Hk]
+    block.qk_norm_rope(a, b, *w, cos, sin, eps=0.0, out=(a, b))
+    assert torch.equal(a, outs[0]) and torch.equal(b, outs[1]) and (room[:, T:] == 7).all() and (room[:, :, Hq + Hk:] == 7).all()
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
 @pytest.mark.parametrize('B,Tq,Tk,H,Hk,D,Dv,causal', [
     (2, 1, 33, 64, 1, 128, 256, False), (1, 3, 65, 64, 1, 8, 8, True), (1, 32, 32, 1, 1, 64, 128, True), (1, 33, 257, 1, 1, 64, 128, True),
     (5, 1, 255, 3, 3, 32, 64, False), (5, 1, 256, 3, 3, 32, 64, False), (2, 1, 513, 3, 3, 32, 256, False), (1, 1, 20000, 2, 1, 16, 24, False),
