@@ -11,10 +11,12 @@ Conventions.  Tensors live on an AMD GPU (there is no CPU path: ``NdHipError``) 
 sums, softmax statistics and products are fp32.  Work is queued on the current stream of the tensors' device, nothing
 synchronises, scratch memory comes from torch's allocator, so a call may be captured into a hipGraph.  Wrong shapes or dtypes
 raise ``ValueError`` / ``TypeError`` before anything is launched.  All three are differentiable (once): gradients flow to
-every floating argument except the tables.  To capture a backward pass, do it on leaves that no graph built outside the
-capture still holds (torch ties a leaf's gradient accumulation to the stream of its first graph).
+every floating argument except the tables; a forward-mode tangent raises ``NotImplementedError``.  To capture a backward pass,
+do it on leaves that no graph built outside the capture still holds (torch ties a leaf's gradient accumulation to the stream of
+its first graph).
 """
 import torch
+import torch.autograd.forward_ad as _fwd
 from torch.autograd.function import once_differentiable
 
 from . import _hip
@@ -35,7 +37,16 @@ def _check(name, t, names, others):
             if o.device != dev:
                 raise ValueError('{} lives on {}, {} on {}'.format(n, o.device, name, dev))
             raise TypeError('{} is {}, {} is {}: one dtype per call'.format(n, o.dtype, name, dtype))
+    if getattr(_fwd, '_current_level', 0) >= 0:                # a level is open, or this torch does not say
+        _no_tangent((name, *names), (t, *others))
     _hip.require_gfx950(dev.index)
+
+
+def _no_tangent(names, tensors):
+    """The operators have no forward-mode derivative, and a launch would drop a tangent as if it were zero."""
+    for n, t in zip(names, tensors):
+        if t is not None and _fwd.unpack_dual(t).tangent is not None:
+            raise NotImplementedError('{} carries a forward-mode tangent: these operators have reverse-mode gradients only'.format(n))
 
 
 class _Nothing(torch.autograd.Function):
@@ -244,6 +255,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
             cos, sin = cos.contiguous(), sin.contiguous()
         if not 0 < 2 * cos.shape[-1] <= D:
             raise ValueError('tables for {} channels, head dim is {}'.format(2 * cos.shape[-1], D))
+        if getattr(_fwd, '_current_level', 0) >= 0:
+            _no_tangent(('cos', 'sin'), (cos, sin))
     _check('q', q, ('k', 'q_weight', 'k_weight'), (k, q_weight, k_weight))
     q, k = _rows(q), _rows(k)
     if out is not None:

@@ -1,0 +1,65 @@
+"""nicediffusion.block as autograd sees its calls, without a GPU: the launch is replaced by a record of its arguments."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from nicediffusion import _hip, block
+
+T4 = (2, 5, 3, 16)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Calls go through to the launch, which notes its name and arguments instead."""
+    made = []
+    monkeypatch.setattr(_hip, 'require_device', lambda t, what='tensor': None)
+    monkeypatch.setattr(_hip, 'require_gfx950', lambda index: None)
+    monkeypatch.setattr(block, '_call', lambda name, device, *args: made.append((name, args)))
+    return made
+
+
+def r(*shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(sum(shape)))
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+QK = dict(q=r(*T4), k=r(*T4), q_weight=r(16), k_weight=r(16))
+DIFF = dict(q=r(2, 5, 4, 32), k=r(2, 7, 2, 32), v=r(2, 7, 2, 24), lambda_q1=r(16), lambda_k1=r(16), lambda_q2=r(16), lambda_k2=r(16))
+FFN = dict(x=r(3, 16), w_in=r(48, 16), w_out=r(16, 24), b_in=r(48), b_out=r(16), residual=r(3, 16))
+EACH = [(f, d, n) for f, d in ((block.qk_norm_rope, QK), (block.differential_attention, DIFF), (block.gated_feed_forward, FFN)) for n in d]
+
+
+@pytest.mark.parametrize('fn,tensors,name', EACH, ids=['{}-{}'.format(f.__name__, n) for f, _, n in EACH])
+@pytest.mark.parametrize('grad', [False, True])
+def test_a_forward_mode_tangent_is_refused(launches, fn, tensors, name, grad):
+    """The operators have no forward-mode derivative: a tangent would be lost, that is, taken for zero."""
+    fn(**tensors)
+    assert launches
+    launches.clear()
+    with fwd.dual_level():
+        given = dict(tensors, **{name: fwd.make_dual(tensors[name], torch.ones_like(tensors[name]))})
+        if grad:
+            given = {n: t.requires_grad_() if n != name and t.is_leaf else t for n, t in ((n, t if n == name else t.clone()) for n, t in given.items())}
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            fn(**given)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match='forward-mode'):
+            fn(**given)
+        fn(**tensors)                                          # a level that is open is no tangent
+    assert len(launches) == 1
+    fn(**tensors)
+
+
+def test_a_forward_mode_tangent_is_refused_for_tables_out_and_empty_calls(launches):
+    cos, sin = r(5, 8), r(5, 8)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for kw in (dict(cos=dual(cos), sin=sin), dict(cos=cos, sin=dual(sin)), dict(out=(dual(r(*T4)), r(*T4))), dict(out=(r(*T4), dual(r(*T4))))):
+            with pytest.raises(NotImplementedError, match='forward-mode'):
+                block.qk_norm_rope(r(*T4), r(*T4), **kw)
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            block.qk_norm_rope(dual(r(2, 0, 3, 16)), r(2, 0, 3, 16))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            block.differential_attention(**dict(DIFF, q=dual(r(2, 0, 4, 32))))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            block.gated_feed_forward(dual(r(0, 16)), r(48, 16), r(16, 24))
+    assert not launches
