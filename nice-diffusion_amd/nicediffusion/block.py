@@ -18,6 +18,7 @@ its first graph).
 import torch
 import torch.autograd.forward_ad as _fwd
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _hip
 
@@ -274,6 +275,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
             raise ValueError('out must be the inputs themselves, in their order, or other memory')
         if q.numel():
             _launch_qk(q, k, q_weight, k_weight, cos, sin, eps, interleaved, qo, ko)
+            increment_version((qo, ko))                        # a graph that saved this memory must not be run backward over it
         return qo, ko
     if _wants_grad(q, k, q_weight, k_weight):
         return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, eps, interleaved)

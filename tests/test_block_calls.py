@@ -63,3 +63,33 @@ def test_a_forward_mode_tangent_is_refused_for_tables_out_and_empty_calls(launch
         with pytest.raises(NotImplementedError, match='forward-mode'):
             block.gated_feed_forward(dual(r(0, 16)), r(48, 16), r(16, 24))
     assert not launches
+
+
+# ------------------------------------------------------------------------------------------------------- writing into out=
+def test_out_is_a_write_that_autograd_sees(launches):
+    """A graph that saved the memory cannot be run backward over what was written there, as after any in-place operation."""
+    x = r(2, 5, 9 * 16).requires_grad_()
+    row = torch.tanh(x)                                        # saved for its own backward
+    q, k = row[..., :48].view(*T4), row[..., 48:96].view(*T4)
+    with torch.no_grad():
+        block.qk_norm_rope(q, k, out=(q, k))
+    assert len(launches) == 1
+    with pytest.raises(RuntimeError, match='inplace operation'):
+        row.sum().backward()
+    x, cache = r(*T4).requires_grad_(), r(2, 8, 3, 16)         # a slot of a cache that a product saved
+    y = x * cache[:, :5]
+    with torch.no_grad():
+        block.qk_norm_rope(r(*T4), r(*T4), out=(r(*T4), cache[:, 3:8]))
+    with pytest.raises(RuntimeError, match='inplace operation'):
+        y.sum().backward()
+
+
+def test_out_counts_each_output_once_per_call_and_skips_what_has_no_counter(launches):
+    a, b = r(*T4), r(*T4)
+    va, vb = a._version, b._version
+    block.qk_norm_rope(r(*T4), r(*T4), out=(a, b))
+    assert (a._version, b._version) == (va + 1, vb + 1)
+    with torch.inference_mode():
+        block.qk_norm_rope(r(*T4), r(*T4), out=(torch.empty(T4), torch.empty(T4)))
+    block.qk_norm_rope(r(2, 0, 3, 16), r(2, 0, 3, 16), out=(r(2, 0, 3, 16), r(2, 0, 3, 16)))
+    assert len(launches) == 2
