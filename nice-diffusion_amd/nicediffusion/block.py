@@ -266,6 +266,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
         qo, ko = out
         for n, o, t in (('out[0]', qo, q), ('out[1]', ko, k)):
             _shape(o, n, *t.shape)
+            if o.requires_grad and torch.is_grad_enabled():
+                raise ValueError('{} requires a gradient, and out= records none: call under torch.no_grad()'.format(n))
             if o.stride(-1) != 1 or 0 in [a for a, z in zip(o.stride(), o.shape) if z > 1]:
                 raise ValueError('{} must have contiguous channels and no rows that repeat'.format(n))
             if o.data_ptr() == t.data_ptr() and _strides(o) != _strides(t):

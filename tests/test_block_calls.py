@@ -93,3 +93,16 @@ def test_out_counts_each_output_once_per_call_and_skips_what_has_no_counter(laun
         block.qk_norm_rope(r(*T4), r(*T4), out=(torch.empty(T4), torch.empty(T4)))
     block.qk_norm_rope(r(2, 0, 3, 16), r(2, 0, 3, 16), out=(r(2, 0, 3, 16), r(2, 0, 3, 16)))
     assert len(launches) == 2
+
+
+def test_out_that_requires_a_gradient_is_refused_in_grad_mode(launches):
+    """As torch's own out=: the write would leave the tensor's history as it was."""
+    leaf, row = r(*T4).requires_grad_(), torch.tanh(r(2, 5, 9 * 16).requires_grad_())
+    part = row[..., :48].view(*T4)
+    for i, out in enumerate(((leaf, r(*T4)), (r(*T4), leaf), (part, r(*T4)), (r(*T4), part))):
+        with pytest.raises(ValueError, match=r'out\[{}\] requires a gradient'.format(i % 2)):
+            block.qk_norm_rope(r(*T4), r(*T4), out=out)
+    assert not launches
+    with torch.no_grad():                                      # a parameter that is set outside of any graph
+        block.qk_norm_rope(r(*T4), r(*T4), out=(leaf, r(*T4)))
+    assert len(launches) == 1 and leaf._version == 1
