@@ -28,7 +28,8 @@ COEF_COLS = 8
 STEP_NO_CLIP = 1
 STEP_PER_IMAGE = 2
 
-# flags of libnd_block.so (mirror include/nd_block.h)
+# flags and codes of libnd_block.so (mirror include/nd_block.h)
+E_ARG = -1
 ROPE_INTERLEAVED = 1
 ATTN_CAUSAL = 1
 ACT_SILU = 0
@@ -175,6 +176,10 @@ class NdHipError(RuntimeError):
     pass
 
 
+class NdArgumentError(NdHipError, ValueError):
+    """libnd_block.so refused an argument (ND_E_ARG): nothing was launched."""
+
+
 def lib_path():
     return _LIB_PATH
 
@@ -238,8 +243,8 @@ def load_block():
 
 def check_block(rc, what=''):
     if rc != 0:
-        raise NdHipError('{} failed (rc={}): {}'.format(what or 'libnd_block call', rc,
-                                                        load_block().nd_block_last_error().decode('utf-8', 'replace')))
+        text = load_block().nd_block_last_error().decode('utf-8', 'replace')
+        raise (NdArgumentError if rc == E_ARG else NdHipError)('{} failed (rc={}): {}'.format(what or 'libnd_block call', rc, text))
 
 
 def build_id():

@@ -106,3 +106,28 @@ def test_out_that_requires_a_gradient_is_refused_in_grad_mode(launches):
     with torch.no_grad():                                      # a parameter that is set outside of any graph
         block.qk_norm_rope(r(*T4), r(*T4), out=(leaf, r(*T4)))
     assert len(launches) == 1 and leaf._version == 1
+
+
+# ------------------------------------------------------------------------------------------------ what the library refuses
+@pytest.fixture
+def no_device(monkeypatch):
+    """Calls reach the library itself, which refuses them before any launch."""
+    monkeypatch.setattr(_hip, 'require_device', lambda t, what='tensor': None)
+    monkeypatch.setattr(_hip, 'require_gfx950', lambda index: None)
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: None)
+    monkeypatch.setattr(block, '_stream', lambda index: None)
+
+
+def test_what_the_library_refuses_is_a_value_error(no_device):
+    """Sizes that only the library looks at: a ValueError like every other wrong shape, and still an NdHipError."""
+    heads = (1 << 18) + 8                                      # a token's heads of 16 channels: more than 2^22 elements
+    q, v = torch.zeros(1, 2, heads, 16), torch.zeros(1, 2, heads, 8)
+    with pytest.raises(ValueError, match='token stride') as e:
+        block.differential_attention(q, q, v, r(8), r(8), r(8), r(8))
+    assert isinstance(e.value, _hip.NdHipError)
+    with pytest.raises(ValueError):
+        _hip.check_block(-1, 'a call')
+    with pytest.raises(_hip.NdHipError) as e:                  # a failed launch is no wrong argument
+        _hip.check_block(-2, 'a call')
+    assert not isinstance(e.value, ValueError)
+    _hip.check_block(0)
