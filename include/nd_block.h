@@ -27,13 +27,18 @@ const char* nd_block_last_error(void); /* thread-local message of the last faili
 
 #define ND_ROPE_INTERLEAVED 1 /* rotated pairs are channels (2i, 2i+1); default: (i, i + R/2) */
 
-/* q [B, T, Hq, D], k [B, T, Hk, D] (Hk may be 0) with element strides (batch, token, head), channels contiguous; outputs may
- * be the inputs themselves (same pointer and strides).  weights [D] or NULL.  cos / sin: fp32 [T][R/2] rows, batch stride
+/* q [B, T, Hq, D], k [B, T, Hk, D] (Hk may be 0) with element strides (batch, token, head), channels contiguous; an output may be
+ * its input itself (same pointer and strides), and overlaps nothing else (refused).  weights [D] or NULL.  cos / sin: fp32 [T][R/2] rows, batch stride
  * table_sb (0 = shared by the batch); the first R channels are rotated (R even, 0 = none).  D even, at most 512. */
 int nd_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
                     const void* q_weight, const void* k_weight, const float* cos, const float* sin, int64_t table_sb, void* q_out,
                     int64_t qo_sb, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh, int B, int T,
                     int Hq, int Hk, int D, int R, float eps, int flags, int dtype, nd_stream_t stream);
+
+/* Whether a [B, T, Ha, D] and b [B, T, Hb, D] (element strides; es: bytes of an element) have an address in common; b NULL: whether
+ * rows of a meet each other.  Exact where both have the same strides (views of one packed row), else 1 if their ranges meet. */
+int nd_rows_overlap(const void* a, int64_t a_sb, int64_t a_st, int64_t a_sh, int Ha, const void* b, int64_t b_sb, int64_t b_st, int64_t b_sh,
+                    int Hb, int B, int T, int D, int es);
 
 /* gradients: dq, dk (own strides) and, where dq_weight / dk_weight is not NULL, the weights' (needs the workspace) */
 int nd_qk_norm_rope_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,

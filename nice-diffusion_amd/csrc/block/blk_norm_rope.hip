@@ -356,9 +356,106 @@ static int norm_rope_check(const char* fn, int B, int T, int Hq, int Hk, int D, 
     return ND_OK;
 }
 
+// Rows of `bytes` bytes at p + sum_i x_i s[i], 0 <= x_i < n[i]
+struct RowBox {
+    uint64_t p;
+    int64_t n[3], s[3], bytes;
+};
+
+static RowBox row_box(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t B, int64_t T, int64_t H, int64_t D, int64_t es) {
+    RowBox r{reinterpret_cast<uintptr_t>(p), {B, T, H}, {sb * es, st * es, sh * es}, D * es};
+    for (int i = 0; i < 3; ++i) {
+        if (r.n[i] == 1) r.s[i] = 0;
+        if (r.s[i] < 0) r.p += (uint64_t)(r.s[i] * (r.n[i] - 1)), r.s[i] = -r.s[i];
+    }
+    return r;
+}
+
+// Is there sum_i x_i s[i] + c = delta with lo[i] <= x_i <= hi[i] and c_lo <= c <= c_hi (and some x_i not 0)?  s descending and
+// positive, so that few x_i are left to try at each level; after `visits` of them the answer is yes.
+static bool row_meet(const int64_t* s, const int64_t* lo, const int64_t* hi, int dims, int64_t delta, int64_t c_lo, int64_t c_hi, bool moved, int& visits) {
+    if (dims == 0) return moved && delta >= c_lo && delta <= c_hi;
+    int64_t r_lo = c_lo, r_hi = c_hi;                          // what the dimensions behind this one reach
+    for (int i = 1; i < dims; ++i) r_lo += lo[i] * s[i], r_hi += hi[i] * s[i];
+    auto div_down = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    int64_t from = -div_down(r_hi - delta, s[0]), to = div_down(delta - r_lo, s[0]);
+    from = from > lo[0] ? from : lo[0];
+    to = to < hi[0] ? to : hi[0];
+    for (int64_t x = from; x <= to; ++x) {
+        if (--visits < 0) return true;
+        if (row_meet(s + 1, lo + 1, hi + 1, dims - 1, delta - x * s[0], c_lo, c_hi, moved || x != 0, visits)) return true;
+    }
+    return false;
+}
+
+// Do the rows of a and b (b null: two rows of a) have a byte in common?  Exact for equal strides; otherwise yes if their ranges meet.
+static bool rows_overlap(const RowBox& a, const RowBox* b) {
+    int64_t s[3], lo[3], hi[3];
+    int dims = 0;
+    if (b) {
+        uint64_t ea = a.p + (uint64_t)a.bytes, eb = b->p + (uint64_t)b->bytes;
+        for (int i = 0; i < 3; ++i) ea += (uint64_t)((a.n[i] - 1) * a.s[i]), eb += (uint64_t)((b->n[i] - 1) * b->s[i]);
+        if (ea <= b->p || eb <= a.p) return false;
+    }
+    for (int i = 0; i < 3; ++i) {
+        const int64_t na = a.n[i], nb = b ? b->n[i] : na, sa = a.s[i], sb = b ? b->s[i] : sa, st = na > 1 ? sa : sb;
+        if (na > 1 && nb > 1 && sa != sb) return true;
+        if (st == 0) {
+            if (!b && na > 1) return true;
+            continue;
+        }
+        int j = dims++;
+        for (; j > 0 && s[j - 1] < st; --j) s[j] = s[j - 1], lo[j] = lo[j - 1], hi[j] = hi[j - 1];
+        s[j] = st, lo[j] = -(nb - 1), hi[j] = na - 1;
+    }
+    int visits = 4096;
+    const int64_t delta = b ? (int64_t)(b->p - a.p) : 0, rb = b ? b->bytes : a.bytes;
+    return row_meet(s, lo, hi, dims, delta, -(rb - 1), a.bytes - 1, b != nullptr, visits);
+}
+
+static bool rows_same(const RowBox& a, const RowBox& b) {
+    for (int i = 0; i < 3; ++i)
+        if (a.n[i] != b.n[i] || a.s[i] != b.s[i]) return false;
+    return a.p == b.p && a.bytes == b.bytes;
+}
+
+// An output may be its own input; any other common address is a race between the workgroups.
+static bool norm_rope_outputs_apart(const NormRopeArgs& a, int es) {
+    RowBox in[2], out[2];
+    const int sides = a.s[1].H ? 2 : 1;
+    for (int i = 0; i < sides; ++i) {
+        const NormRopeSide& s = a.s[i];
+        in[i] = row_box(s.x, s.xb, s.xt, s.xh, a.B, a.T, s.H, a.D, es);
+        out[i] = row_box(s.out, s.ob, s.ot, s.oh, a.B, a.T, s.H, a.D, es);
+    }
+    if (sides == 2 && rows_overlap(out[0], &out[1])) return false;
+    for (int i = 0; i < sides; ++i) {
+        if (rows_overlap(out[i], nullptr)) return false;
+        for (int j = 0; j < sides; ++j) {
+            if (!(i == j && rows_same(out[i], in[j])) && !(i != j && rows_same(out[j], in[j])) && rows_overlap(out[i], &in[j])) return false;
+            const RowBox w = row_box(a.s[j].w, 0, 0, 0, 1, 1, 1, a.D, es);
+            if (a.s[j].w && rows_overlap(out[i], &w)) return false;
+        }
+        for (const float* t : {a.cos, a.sin}) {
+            const RowBox c = row_box(t, a.cb, a.R / 2, 0, a.B, a.T, 1, a.R / 2, 4);
+            if (a.R && rows_overlap(out[i], &c)) return false;
+        }
+    }
+    return true;
+}
+
 }  // namespace ndb
 
 using namespace ndb;
+
+extern "C" int nd_rows_overlap(const void* a, int64_t a_sb, int64_t a_st, int64_t a_sh, int Ha, const void* b, int64_t b_sb, int64_t b_st,
+                               int64_t b_sh, int Hb, int B, int T, int D, int es) {
+    if (B <= 0 || T <= 0 || D <= 0 || es <= 0 || Ha <= 0 || (b && Hb <= 0)) return 0;
+    const RowBox x = row_box(a, a_sb, a_st, a_sh, B, T, Ha, D, es);
+    if (!b) return rows_overlap(x, nullptr);
+    const RowBox y = row_box(b, b_sb, b_st, b_sh, B, T, Hb, D, es);
+    return rows_overlap(x, &y);
+}
 
 extern "C" int nd_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
                                int64_t k_sh, const void* q_weight, const void* k_weight, const float* cos, const float* sin,
@@ -374,6 +471,7 @@ extern "C" int nd_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_st, int64_
     a.cos = cos, a.sin = sin, a.cb = table_sb;
     a.B = B, a.T = T, a.D = D, a.R = R, a.eps = eps;
     a.rows = (long)B * T * (Hq + Hk);
+    NDB_REQUIRE(norm_rope_outputs_apart(a, dtype == ND_DT_BF16 ? 2 : 4), fn, "outputs overlap each other, themselves or what is read (other than their own input)");
     const bool inter = flags & ND_ROPE_INTERLEAVED;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (dtype == ND_DT_BF16)

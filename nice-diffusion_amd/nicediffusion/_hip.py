@@ -152,6 +152,7 @@ BLOCK_SIGNATURES = {
     'nd_block_build_id': ([], ctypes.c_char_p),
     'nd_block_last_error': ([], ctypes.c_char_p),
     'nd_qk_norm_rope': (_T3 * 2 + [_vp, _vp, _vp, _vp, _i64] + _T3 * 2 + [_i] * 6 + [_f, _i, _i, _vp], _i),
+    'nd_rows_overlap': ((_T3 + [_i]) * 2 + [_i] * 4, _i),
     'nd_qk_norm_rope_bwd': (_T3 * 2 + [_vp, _vp, _vp, _vp, _i64] + _T3 * 4 + [_vp, _vp, _vp] + [_i] * 6 + [_f, _i, _i, _vp], _i),
     'nd_qk_norm_rope_bwd_workspace_floats': ([_i] * 5, _i64),
     'nd_diff_attention': (_T3 * 3 + [_vp] * 4 + [_i64, _f] + [_vp] * 6 + [_i] * 7 + [_f, _i, _i, _vp], _i),

@@ -225,7 +225,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
     rotated, the rest only normed; None: norm alone.  Pairs are channels (i, i + R/2), or (2i, 2i + 1) if ``interleaved``.
 
     Returns new contiguous (q, k).  ``out=(q_out, k_out)`` writes there instead and records no gradient: the inputs themselves
-    (in place in the packed row that ``nd_attention_nhwc`` reads) or memory that does not overlap them (a slot of a cache)."""
+    (in place in the packed row that ``nd_attention_nhwc`` reads) or memory that shares no address with them, the tables, the
+    weights or each other (a slot of a cache; where address ranges interleave, equal strides are needed to tell): else ValueError."""
     if q.dim() != 4:
         raise ValueError('q has shape {}, expected [B, T, heads, D]'.format(tuple(q.shape)))
     B, T, Hq, D = q.shape

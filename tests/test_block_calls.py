@@ -131,3 +131,75 @@ def test_what_the_library_refuses_is_a_value_error(no_device):
         _hip.check_block(-2, 'a call')
     assert not isinstance(e.value, ValueError)
     _hip.check_block(0)
+
+
+def touched(base, strides, heads, B, T, D):
+    """The element addresses of a [B, T, heads, D] tensor, one set per row."""
+    sb, st, sh = strides
+    return [set(range(base + b * sb + t * st + h * sh, base + b * sb + t * st + h * sh + D)) for b in range(B) for t in range(T) for h in range(heads)]
+
+
+def test_rows_overlap_against_every_address():
+    """nd_rows_overlap against the sets of addresses themselves: views of packed rows, slots, repeats and strides at random; where two
+    layouts that interleave have different strides it may say yes without need, never no."""
+    import random
+    lib, rng, es, far = _hip.load_block(), random.Random(1), 4, 1 << 20
+    seen = {(w, g): 0 for w in (0, 1) for g in (0, 1)}
+    for n in range(6000):
+        B, T, D = rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 4)
+        Ha, Hb = rng.randint(1, 3), rng.randint(1, 3)
+        sh = rng.choice([D, D, D + 1, 2 * D, 3 * D])
+        st = rng.choice([3 * sh, 4 * sh, 6 * sh, sh * max(Ha, Hb) + rng.randint(0, 5), rng.randint(0, 30)])
+        sb = rng.choice([T * st, (T + 2) * st, 0, rng.randint(0, 90)])
+        same = rng.random() < 0.8
+        sa = (sb, st, sh)
+        sb2 = sa if same else (rng.randint(0, 90), rng.randint(0, 30), rng.choice([D, 2 * D]))
+        off = rng.choice([0, D, Ha * sh, st, rng.randint(0, 60), rng.randint(0, 400)])
+        a, b = touched(0, sa, Ha, B, T, D), touched(off, sb2, Hb, B, T, D)
+        want = int(bool(set().union(*a) & set().union(*b)))
+        got = lib.nd_rows_overlap(far, *sa, Ha, far + off * es, *sb2, Hb, B, T, D, es)
+        assert got == lib.nd_rows_overlap(far + off * es, *sb2, Hb, far, *sa, Ha, B, T, D, es)
+        assert got >= want, (sa, sb2, Ha, Hb, B, T, D, off)
+        if same:
+            assert got == want, (sa, Ha, Hb, B, T, D, off)
+        seen[want, got] += 1
+        alone = int(sum(len(s) for s in a) != len(set().union(*a)))        # rows of one tensor that meet each other
+        assert lib.nd_rows_overlap(far, *sa, Ha, None, 0, 0, 0, 0, B, T, D, es) == alone, (sa, Ha, B, T, D)
+    assert seen[0, 0] > 500 and seen[1, 1] > 500
+
+
+def test_out_that_overlaps_is_refused(no_device):
+    """Neither a shifted view of the inputs' rows nor one of the other input, a weight, a table or the other output may be written."""
+    base, fresh, fresh2 = r(2, 9, 9, 16), r(*T4), r(*T4)
+    part = lambda h, t=0: base[:, t:t + 5, h:h + 3]  # noqa: E731
+    q, k = part(0), part(3)
+    halves = base.flatten()[8:8 + 5 * 144 + 9 * 144].as_strided(T4, (9 * 144, 144, 16, 1))      # half a head further
+    for out in ((part(1), fresh), (part(0, 1), part(3)), (q, part(4)), (part(2), k), (fresh, part(2)), (q, part(1)), (part(5), part(6)), (part(4), fresh),
+                (halves, fresh), (fresh, part(0)), (part(3, 1), fresh)):
+        with pytest.raises(ValueError, match='overlap'):
+            block.qk_norm_rope(q, k, out=out)
+    with pytest.raises(ValueError, match='overlap'):           # rows that meet each other
+        block.qk_norm_rope(q, k, out=(torch.as_strided(r(2000), T4, (240, 48, 8, 1)), fresh))
+    weight, flat = fresh[1, 2, 1], torch.cat([r(5, 8).flatten(), r(440)])
+    table = flat.as_strided((5, 8), (8, 1))
+    for kw, out in ((dict(q_weight=weight), (fresh, fresh2)), (dict(k_weight=weight), (fresh, fresh2)), (dict(cos=table, sin=r(5, 8)), (fresh, flat.view(T4))),
+                    (dict(cos=r(5, 8), sin=table), (flat.view(T4), fresh))):
+        with pytest.raises(ValueError, match='overlap'):
+            block.qk_norm_rope(q, k, out=out, **kw)
+
+
+def test_layouts_that_only_interleave_do_not_overlap():
+    """The q and k columns of one packed row, per-head q | k | v, a cache slot beside others, a batch of one."""
+    lib, D, es, far = _hip.load_block(), 16, 2, 1 << 20
+    at = lambda i: far + i * es  # noqa: E731
+    row = (7 * 144, 144, D)
+    assert lib.nd_rows_overlap(at(0), *row, 3, at(3 * D), *row, 3, 2, 7, D, es) == 0
+    assert lib.nd_rows_overlap(at(0), *row, 5, at(5 * D), *row, 2, 2, 7, D, es) == 0
+    assert lib.nd_rows_overlap(at(0), *row, 5, at(4 * D), *row, 2, 2, 7, D, es) == 1
+    assert lib.nd_rows_overlap(at(0), 7 * 144, 144, 3 * D, 3, at(D), 7 * 144, 144, 3 * D, 3, 2, 7, D, es) == 0
+    assert lib.nd_rows_overlap(at(0), 0, 144, 0, 1, at(D), 0, 144, D, 4, 1, 7, D, es) == 0           # strides that say nothing are 0
+    slot = (50 * 2 * D, 2 * D, D)
+    assert lib.nd_rows_overlap(at(4 * 2 * D), *slot, 2, at(5 * 2 * D), *slot, 2, 3, 1, D, es) == 0
+    assert lib.nd_rows_overlap(at(4 * 2 * D), *slot, 2, at(5 * 2 * D), *slot, 2, 3, 2, D, es) == 1
+    assert lib.nd_rows_overlap(at(0), 1 << 40, 1 << 30, D, 3, at(3 * D), 1 << 40, 1 << 30, D, 3, 64, 512, D, es) == 0
+    assert lib.nd_rows_overlap(at(0), -7 * 144, 144, D, 3, at(-7 * 144), 0, 144, D, 3, 2, 7, D, es) == 1      # a negative stride
