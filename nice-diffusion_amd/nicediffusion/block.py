@@ -271,11 +271,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None, eps=1e-
                 raise ValueError('{} requires a gradient, and out= records none: call under torch.no_grad()'.format(n))
             if o.stride(-1) != 1 or 0 in [a for a, z in zip(o.stride(), o.shape) if z > 1]:
                 raise ValueError('{} must have contiguous channels and no rows that repeat'.format(n))
-            if o.data_ptr() == t.data_ptr() and _strides(o) != _strides(t):
-                raise ValueError('{} begins where its input does but lies differently'.format(n))
         _check('q', q, ('out[0]', 'out[1]'), (qo, ko))
-        if q.numel() and qo.data_ptr() in (k.data_ptr(), ko.data_ptr()) or k.numel() and ko.data_ptr() == q.data_ptr():
-            raise ValueError('out must be the inputs themselves, in their order, or other memory')
         if q.numel():
             _launch_qk(q, k, q_weight, k_weight, cos, sin, eps, interleaved, qo, ko)
             increment_version((qo, ko))                        # a graph that saved this memory must not be run backward over it
