@@ -46,6 +46,9 @@ inline int ensure_max_lds(const void* kern, bool (&flags)[kMaxDevices], const ch
         if (!(cond)) return ndb::fail_arg(fn, msg); \
     } while (0)
 
+// a launch counts its threads in 32 bits
+inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads < (1LL << 32); }
+
 inline bool aligned_to(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -545,6 +545,8 @@ int diff_head_dim(int D, int Dv) {
     return n <= 32 ? 32 : (n <= 64 ? 64 : 128);
 }
 
+int diff_bwd_check(const char* fn, const DiffArgs& a, int dtype);      // blk_diff_attn_bwd.hip
+
 struct DiffPlan {
     bool few;
     int splits, chunk;
@@ -676,6 +678,7 @@ extern "C" int nd_diff_attention(const void* q, int64_t q_sb, int64_t q_st, int6
     if (int rc = diff_check(fn, a, dtype)) return rc;
     a.g = H / Hk;
     NDB_REQUIRE(out && aligned_to(out, 16) && (!out1 || (out2 && lse && aligned_to(out1, 16) && aligned_to(out2, 16))), fn, "outputs missing or not 16-byte aligned");
+    if (int rc = lse ? diff_bwd_check(fn, a, dtype) : ND_OK) return rc;
     const DiffPlan pl = diff_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4, a.causal);
     a.splits = pl.splits, a.chunk = pl.chunk;
     NDB_REQUIRE(pl.splits == 1 || (workspace && aligned_to(workspace, 16)), fn, "workspace missing");

@@ -563,6 +563,17 @@ static DiffBwdPlan diff_bwd_plan(int B, int Tq, int Tk, int H, int Hk, int D, in
     return pl;
 }
 
+// What a backward pass of these sizes needs beyond diff_check; a forward pass that keeps its statistics asks too, so that no step
+// ends between the two.  The output's gradient may come contiguous, with token rows of H Dv elements.
+int diff_bwd_check(const char* fn, const DiffArgs& a, int dtype) {
+    const DiffBwdPlan pl = diff_bwd_plan(a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.Dv, dtype == ND_DT_BF16 ? 2 : 4, a.causal);
+    const int64_t units = (int64_t)a.B * a.Hk, tiles = ((int64_t)a.Tq * (a.H / a.Hk) + 127) / 128;
+    NDB_REQUIRE(grid_fits(units * pl.key_blocks * pl.row_splits, 64 * pl.waves) && grid_fits(units * tiles * pl.key_splits, 256), fn,
+                "too many workgroups for one launch of the backward pass");
+    NDB_REQUIRE(a.Tq == 1 || (int64_t)a.H * a.Dv <= (1 << 22), fn, "the output's gradient: more than 2^22 elements a token");
+    return ND_OK;
+}
+
 template <typename T>
 static int dispatch_diff_bwd(const char* fn, const DiffBwdArgs& a, hipStream_t st) {
     switch (diff_head_dim(a.f.D, a.f.Dv)) {
@@ -603,6 +614,7 @@ extern "C" int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, 
     a.B = B, a.Tq = Tq, a.Tk = Tk, a.H = H, a.Hk = Hk, a.D = D, a.Dv = Dv, a.causal = flags & ND_ATTN_CAUSAL;
     a.scale = scale, a.c = scale * 1.4426950408889634f;
     if (int rc = diff_check(fn, a, dtype)) return rc;
+    if (int rc = diff_bwd_check(fn, a, dtype)) return rc;
     a.g = H / Hk;
     NDB_REQUIRE(out1 && out2 && lse && dout && dq && dk && dv && workspace, fn, "null pointer");
     const int per = dtype == ND_DT_BF16 ? 8 : 4;
@@ -611,7 +623,6 @@ extern "C" int nd_diff_attention_bwd(const void* q, int64_t q_sb, int64_t q_st, 
     NDB_REQUIRE(aligned_to(out1, 16) && aligned_to(out2, 16) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16), fn, "pointers must be 16-byte aligned");
     const DiffBwdPlan pl = diff_bwd_plan(B, Tq, Tk, H, Hk, D, Dv, dtype == ND_DT_BF16 ? 2 : 4, a.causal);
     p.waves = pl.waves, p.key_blocks = pl.key_blocks, p.row_splits = pl.row_splits, p.key_splits = pl.key_splits, p.chunk = pl.chunk;
-    NDB_REQUIRE((int64_t)B * Hk * p.key_blocks <= (1 << 20) && (int64_t)B * Hk * (((int64_t)Tq * a.g + 127) / 128) <= (1 << 20), fn, "too many workgroups for one launch");
     NDB_REQUIRE(aligned_to(workspace, 16), fn, "workspace must be 16-byte aligned");
     p.dout = {dout, do_sb, do_st, do_sh};
     p.o1 = out1, p.o2 = out2, p.lse = lse, p.dq = dq, p.dk = dk, p.dv = dv;

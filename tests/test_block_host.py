@@ -232,3 +232,19 @@ def test_rotary_table_values():
 def test_rotary_table_refuses(pos, ch):
     with pytest.raises(ValueError):
         block.rotary_table(pos, ch)
+
+
+def diff_bwd_args(**kw):
+    d = diff_args(**dict(dict(o1=A, o2=A, lse=A), **kw))
+    tensors, (out1, out2, lse, ws), sizes = d[:19], d[20:24], d[24:]
+    dout = (A, *kw.get('dos', (640, 128, 64)))
+    return (*tensors, out1, out2, lse, *dout, A, A, A, None, None, None, None, ws, *sizes)
+
+
+@pytest.mark.parametrize('kw,what', [
+    (dict(B=1 << 21, H=8, Hk=8, Tq=1, Tk=1), 'workgroups'), (dict(B=1 << 12, H=1, Hk=1, D=8, Dv=8, Tq=1, Tk=1 << 20), 'workgroups'),
+    (dict(B=1, H=1 << 17, Hk=1 << 17, D=8, Dv=64, Tq=2, Tk=1, qs=(0, 1 << 21, 16)), 'gradient'),
+])
+def test_a_forward_pass_that_is_kept_refuses_what_its_backward_pass_would(kw, what):
+    refused('nd_diff_attention_bwd', diff_bwd_args(**kw), what)
+    refused('nd_diff_attention', diff_args(o1=A, o2=A, lse=A, **kw), what)

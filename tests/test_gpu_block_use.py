@@ -472,3 +472,35 @@ def test_differential_attention_without_keys_ignores_its_queries():
     q = torch.full((2, 3, 2, 16), math.inf, device=DEV).requires_grad_()
     o = block.differential_attention(q, torch.empty(2, 0, 2, 16, device=DEV), torch.empty(2, 0, 2, 16, device=DEV), *lams)
     assert (o == 0).all() and (torch.autograd.grad(o.sum(), q)[0] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------------------- many short sequences
+def test_differential_attention_of_more_than_2_20_short_sequences():
+    """Windows: 2^20 + 8 (sequence, key head)s of three tokens.  The first and the last sequences against the definition, the vectors'
+    gradients against the sum over all of them."""
+    B, T, H, D, Dv = (1 << 17) + 1, 3, 8, 8, 16
+    g = torch.Generator(DEV).manual_seed(1)
+    q, k, v, dout = (torch.randn(B, T, H, n, device=DEV, generator=g).to(BF) for n in (2 * D, 2 * D, Dv, Dv))
+    lams = [rnd(D, seed=4 + i, dtype=BF, scale=0.2) for i in range(4)]
+    leaves = [t.requires_grad_() for t in (q, k, v, *lams)]
+    out = block.differential_attention(*leaves, causal=True)
+    grads = torch.autograd.grad(out, leaves, dout)
+    wide = [t.detach().double() for t in lams]
+    for s in (slice(0, 20), slice(B - 20, B)):
+        (ref, err), want = diff_ref(*(t.detach()[s].double() for t in (q, k, v)), wide, 0.8, D ** -0.5, (T,) * 20, True, half_ulp(BF), dout[s].double())
+        assert within(out[s], ref, err, BF)
+        for got, (r, e) in zip(grads[:3], want):
+            assert within(got[s], r, e, BF)
+    a, b, vv, do = (t.detach().double().transpose(1, 2) for t in (q[..., D:], k[..., D:], v, dout))
+    x = (a @ b.transpose(-1, -2).contiguous()) * D ** -0.5
+    smax = x.abs().max().item()
+    p2 = torch.softmax(x.masked_fill(torch.ones(T, T, dtype=torch.bool, device=DEV).triu(1), -math.inf), -1)
+    terms = p2 * (do @ vv.transpose(-1, -2).contiguous())
+    # dlam = -sum P2 dP: P2 off by eps (as in diff_ref), dP by its sum over Dv channels, then fp32 sums whose longest chain is one of
+    # 1024 threads over four waves' partials of every (sequence, head)
+    eps = (smax + 8) * 4 * half_ulp(F32) * math.sqrt(D)
+    size = (p2 * (do.abs() @ vv.abs().transpose(-1, -2).contiguous())).sum()
+    e_lam = (eps + 4 * math.sqrt(Dv) * half_ulp(F32) + fp32_tol(4 * B * H / 1024 + 100)) * size
+    x1, x2 = (wide[0] * wide[1]).sum().exp(), (wide[2] * wide[3]).sum().exp()
+    for got, val, o in zip(grads[3:], (x1, x1, -x2, -x2), (wide[1], wide[0], wide[3], wide[2])):
+        assert within(got, -terms.sum() * val * o, e_lam * val.abs() * o.abs(), BF)
