@@ -607,7 +607,7 @@ static int launch_diff(const char* fn, const DiffArgs& a, bool few, hipStream_t 
     const int rows = a.Tq * a.g, per = few ? 16 : 128;
     const int vblocks = (a.Dv + DiffShape<T, HD>::DV - 1) / DiffShape<T, HD>::DV;
     const int64_t blocks = (int64_t)a.B * a.Hk * ((rows + per - 1) / per) * a.splits * vblocks;
-    NDB_REQUIRE(blocks <= (1 << 24), fn, "too many workgroups for one launch");
+    NDB_REQUIRE(grid_fits(blocks, few ? 64 * DiffShape<T, HD>::NW_FEW : 256), fn, "too many workgroups for one launch");
     if (few) hipLaunchKernelGGL((diff_few_kernel<T, HD>), dim3((unsigned)blocks), dim3(64 * DiffShape<T, HD>::NW_FEW), 0, st, a);
     else hipLaunchKernelGGL((diff_attn_kernel<T, HD>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     if (a.splits > 1) {

@@ -399,6 +399,7 @@ static Plan plan_gemm(int64_t M, int64_t N, int64_t K, int es, bool gated, bool 
             const int64_t per = (stages + want - 1) / want;
             const int64_t splits = (stages + per - 1) / per;
             if (want > 1 && (per < 4 || splits * M * N > (1LL << 28))) break;
+            if (ti < 4 && !grid_fits(tiles * splits, GEMM_THREADS)) break;
             const int64_t each = (tiles * splits + 255) / 256, rounds = (each + 4 / ti - 1) / (4 / ti);      // workgroups a CU
             const double work = (double)each * per * stage, wait = (double)rounds * per * 850.0;
             double t = (work > wait ? work : wait) + (double)rounds * (ti == 4 ? 8200.0 : (ti == 2 ? 4600.0 : 2600.0)) + epilogue;
@@ -423,7 +424,7 @@ static int launch_gemm(const char* fn, const GemmSide<T>& x, const GemmSide<T>& 
     const int per_n = gate ? tile / 2 : tile, cols = gate ? gate : w.n;
     a.tiles_n = (cols + per_n - 1) / per_n;
     const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n * pl.splits;
-    NDB_REQUIRE(blocks <= (1 << 24), fn, "too many tiles for one launch");
+    NDB_REQUIRE(grid_fits(blocks, GEMM_THREADS), fn, "too many tiles for one launch");
     auto kern = gemm_kernel<T, TI, XK, WK, Epi>;
     static bool attr_set[kMaxDevices] = {};
     if (int rc = ensure_max_lds(reinterpret_cast<const void*>(kern), attr_set, fn)) return rc;
@@ -537,6 +538,7 @@ static int ffn_backward(const char* fn, const FfnBwd<T>& a, hipStream_t st) {
 
 static int ffn_check(const char* fn, int M, int C, int F, int act, int dtype) {
     NDB_REQUIRE(M > 0 && C > 0 && F > 0, fn, "sizes must be positive");
+    NDB_REQUIRE(M <= (1 << 30), fn, "more than 2^30 rows");      // a row index and the step behind it fit 32 bits
     NDB_REQUIRE(C % 8 == 0 && F % 8 == 0, fn, "channels and hidden channels must be multiples of 8");
     NDB_REQUIRE((int64_t)C * F <= (1LL << 28) && C <= (1 << 20) && F <= (1 << 20), fn, "weights of more than 2^28 elements, or more than 2^20 channels");
     NDB_REQUIRE(act >= ND_ACT_SILU && act <= ND_ACT_GELU_TANH, fn, "unknown activation");

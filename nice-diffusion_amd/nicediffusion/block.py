@@ -493,8 +493,8 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, residual=None, act
         _shape(b_out, 'b_out', C)
     if residual is not None:
         _shape(residual, 'residual', *x.shape)
-    if x.numel() // C >= 1 << 31:
-        raise ValueError('too many rows')
+    if x.numel() // C > 1 << 30:
+        raise ValueError('more than 2^30 rows')
     _check('x', x, ('w_in', 'w_out', 'b_in', 'b_out', 'residual'), (w_in, w_out, b_in, b_out, residual))
     act = _ACTS[activation]
     if _wants_grad(x, w_in, b_in, w_out, b_out, residual):

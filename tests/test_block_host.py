@@ -248,3 +248,22 @@ def diff_bwd_args(**kw):
 def test_a_forward_pass_that_is_kept_refuses_what_its_backward_pass_would(kw, what):
     refused('nd_diff_attention_bwd', diff_bwd_args(**kw), what)
     refused('nd_diff_attention', diff_args(o1=A, o2=A, lse=A, **kw), what)
+
+
+def test_sizes_past_what_a_launch_can_count_are_refused():
+    """Few rows run in workgroups of 512 threads: 2^23 of them are 2^32 threads.  A feed-forward row index and its step stay in 32 bits."""
+    refused('nd_diff_attention', diff_args(B=1 << 20, H=8, Hk=8, Tq=1, Tk=1), 'workgroups')
+    refused('nd_gated_ffn', ffn_args(M=(1 << 30) + 1), '2\\^30 rows')
+    refused('nd_gated_ffn_bwd', (A, 64, A, 64, A, A, A, A, A, A, None, A, None, A, A, (1 << 30) + 1, 64, 128, 0, _hip.DT_F32, None), '2\\^30 rows')
+    with pytest.raises(ValueError, match='2\\^30 rows'):
+        block.gated_feed_forward(torch.zeros(1, 8).expand((1 << 30) + 1, 8), z(16, 8), z(8, 8))
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason='the call would be launched')
+@pytest.mark.parametrize('C,F', [(8, 8), (64, 256), (256, 64), (72, 24)])
+@pytest.mark.parametrize('M', [(1 << 26) + 1, 1 << 30])
+def test_every_accepted_row_count_has_a_tile_that_fits_a_launch(M, C, F):
+    lib = _hip.load_block()
+    for dtype in (_hip.DT_BF16, _hip.DT_F32):
+        assert lib.nd_gated_ffn(*ffn_args(M=M, C=C, F=F, ldx=C, ldy=C, dtype=dtype)) == -2, lib.nd_block_last_error()
+        assert lib.nd_gated_ffn_bwd_workspace_floats(M, C, F, dtype) > 0
