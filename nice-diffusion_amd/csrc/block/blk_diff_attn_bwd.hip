@@ -255,6 +255,15 @@ __global__ void __launch_bounds__(64 * NW, (HD * (int)sizeof(T) == 64 ? 3 : (HD 
             if (h < hg0 || h > hg1) p.dlam_part[((int64_t)at_part * NW + wave) * f.g + h] = 0.f;
     }
     if (key >= f.Tk) return;
+    if (!kin) {                                               // its weights are zero, but zero times a row's NaN is none
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+#pragma unroll
+            for (int d = 0; d < (DK ? HD / 32 : 1); ++d) dk[0][d][e] = dk[1][d][e] = 0.f;
+#pragma unroll
+            for (int d = 0; d < (DVG ? S::DV / 32 : 1); ++d) dv[d][e] = 0.f;
+        }
+    }
     const int64_t krow = ((int64_t)b * f.Tk + key) * f.Hk + hk;
     const float scale = p.row_splits > 1 ? 1.f : (len == 1 ? 0.f : f.scale);
     float* const part = p.part_kv + ((int64_t)rs * f.B * f.Tk * f.Hk + krow) * (2 * f.D + f.Dv);

@@ -355,9 +355,10 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
     of a packed qkv row); a cache that is longer than its contents is passed whole with ``key_lengths``.  The lambda vectors are [D]
     (one layer's) or [H, D] (each head its own).  scale defaults to D ** -0.5 and must be positive.
 
-    key_lengths [B] (int32 or int64, on the GPU): keys at or past it take no part, whatever their memory holds; values are held
-    to 0 .. Tk.  causal: query t sees the keys up to t + length - Tq (the queries are the sequence's last).  A query that sees no
-    key gives a zero row and no gradient.  Returns [B, Tq, H, Dv], contiguous.  Few query rows (Tq H / Hk <= 32, single tokens) have
+    key_lengths [B] (int32 or int64, on the GPU): keys at or past it take no part, whatever their memory holds, and get zero
+    gradients; values are held to 0 .. Tk.  causal: query t sees the keys up to t + length - Tq (the queries are the sequence's
+    last); it hides by weights of zero, so a NaN or infinite key or value may spoil rows before it too.  A query that sees no key
+    gives a zero row and no gradient.  Returns [B, Tq, H, Dv], contiguous.  Few query rows (Tq H / Hk <= 32, single tokens) have
     a form of their own that divides the keys."""
     if q.dim() != 4 or q.shape[3] % 2:
         raise ValueError('q has shape {}, expected [B, Tq, H, 2 D]'.format(tuple(q.shape)))

@@ -504,3 +504,34 @@ def test_differential_attention_of_more_than_2_20_short_sequences():
     x1, x2 = (wide[0] * wide[1]).sum().exp(), (wide[2] * wide[3]).sum().exp()
     for got, val, o in zip(grads[3:], (x1, x1, -x2, -x2), (wide[1], wide[0], wide[3], wide[2])):
         assert within(got, -terms.sum() * val * o, e_lam * val.abs() * o.abs(), BF)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('B,T,H,Hk,D,Dv', [(2, 70, 2, 2, 32, 64), (2, 300, 2, 1, 64, 128), (1, 40, 1, 1, 128, 256), (1, 2000, 1, 1, 64, 128), (48, 600, 8, 8, 40, 64)])
+def test_gradients_past_a_sequences_end_are_zero_whatever_the_queries_hold(B, T, H, Hk, D, Dv, dtype):
+    """Keys behind a sequence's end take no part: their gradients are zero beside NaN and infinite queries and output gradients too, the
+    other queries' are right, and another sequence's are as they were."""
+    q, k, v = rnd(B, T, H, 2 * D, seed=1, dtype=dtype), rnd(B, T, Hk, 2 * D, seed=2, dtype=dtype), rnd(B, T, Hk, Dv, seed=3, dtype=dtype)
+    lams = [rnd(D, seed=4 + i, dtype=dtype, scale=0.2) for i in range(4)]
+    dout = rnd(B, T, H, Dv, seed=9, dtype=dtype)
+    n = T // 2 + 3
+    ln = torch.tensor([n] * B, device=DEV)
+
+    def grads(q, dout):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v, *lams)]
+        return torch.autograd.grad(block.differential_attention(*leaves, key_lengths=ln), leaves, dout)
+
+    good = grads(q, dout)
+    _, want = diff_ref(*(t[:1].double() for t in (q, k, v)), [t.double() for t in lams], 0.8, D ** -0.5, (n,), False, half_ulp(BF) if dtype == BF else 0.0, dout[:1].double())
+    for bad in ('query', 'gradient'):
+        q2, d2 = q.clone(), dout.clone()
+        (q2 if bad == 'query' else d2)[0, 5, 0, 3] = math.nan
+        (q2 if bad == 'query' else d2)[0, 9, 0, 7] = math.inf
+        dq, dk, dv, *_ = grads(q2, d2)
+        assert (dk[:, n:] == 0).all() and (dv[:, n:] == 0).all(), bad
+        assert torch.isnan(dk[0, :n]).any() and torch.isnan(dq[0, 5, 0]).any()
+        rest = [t for t in range(T) if t not in (5, 9)]
+        # other rows of the wave may take another reference for their weights, so they agree within their own bounds
+        assert within(dq[:1, rest], want[0][0][:, rest], want[0][1][:, rest], dtype)
+        for a, b in zip((dq, dk, dv), good):
+            assert torch.equal(a[1:], b[1:])
