@@ -432,7 +432,9 @@ class _GatedFfn(torch.autograd.Function):
         xm, wi, wo = _matrix(x, C), _aligned(w_in), _aligned(w_out)
         rm = xm if res is x else (None if res is None else _matrix(res, C))
         if xm.shape[0]:
-            y, h, au = _launch_ffn(xm, wi, _aligned(b_in), wo, _aligned(b_out), rm, act, True, x.shape)
+            need = ctx.needs_input_grad
+            y, h, au = _launch_ffn(xm, wi, _aligned(b_in), wo, _aligned(b_out), rm, act, any(need[:3]), x.shape)
+            h = h if need[3] else None                         # what no gradient wanted here is made from is not held
         else:
             y, h, au = xm.new_empty(x.shape), None, None
         ctx.save_for_backward(xm, wi, wo, h, au)
@@ -457,8 +459,8 @@ class _GatedFfn(torch.autograd.Function):
                 g = _matrix(dy, C)
                 dau = torch.empty(M, 2 * F, **new) if any(need[:3]) else None
                 ws = _floats(_hip.load_block().nd_gated_ffn_bwd_workspace_floats(M, C, F, _DT[x.dtype]), x.device)
-                _call('nd_gated_ffn_bwd', x.device, g.data_ptr(), _ld(g), x.data_ptr(), _ld(x), w_in.data_ptr(), w_out.data_ptr(), au.data_ptr(),
-                      h.data_ptr(), _ptr(dx), _ptr(dwi), _ptr(dbi), _ptr(dwo), _ptr(dbo), _ptr(dau), _ptr(ws), M, C,
+                _call('nd_gated_ffn_bwd', x.device, g.data_ptr(), _ld(g), x.data_ptr(), _ld(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(au),
+                      _ptr(h), _ptr(dx), _ptr(dwi), _ptr(dbi), _ptr(dwo), _ptr(dbo), _ptr(dau), _ptr(ws), M, C,
                       F, ctx.act, _DT[x.dtype])
         else:
             for t in (dwi, dbi, dwo, dbo):
@@ -473,7 +475,7 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, residual=None, act
     x [..., C]; w_in [2F, C]: the gate's rows Wg, then the up projection's Wu; w_out [C, F]; b_in [2F], b_out [C], residual
     (x's shape) or None.  C and F multiples of 8.  activation: 'silu', 'gelu' (error function) or 'gelu_tanh'.  Returns a new
     contiguous tensor of x's shape.  In bfloat16 the hidden row is rounded once between the two products; a backward pass keeps
-    it and the pre-activations (3 F values a token)."""
+    it for w_out's gradient and the pre-activations for those of x, w_in and b_in (3 F values a token for all)."""
     if activation not in _ACTS:
         raise ValueError('activation is {!r}, expected one of {}'.format(activation, sorted(_ACTS)))
     if x.dim() < 1:

@@ -203,3 +203,20 @@ def test_layouts_that_only_interleave_do_not_overlap():
     assert lib.nd_rows_overlap(at(4 * 2 * D), *slot, 2, at(5 * 2 * D), *slot, 2, 3, 2, D, es) == 1
     assert lib.nd_rows_overlap(at(0), 1 << 40, 1 << 30, D, 3, at(3 * D), 1 << 40, 1 << 30, D, 3, 64, 512, D, es) == 0
     assert lib.nd_rows_overlap(at(0), -7 * 144, 144, D, 3, at(-7 * 144), 0, 144, D, 3, 2, 7, D, es) == 1      # a negative stride
+
+
+# --------------------------------------------------------------------------------------------------------- partial gradients
+def test_the_feed_forward_holds_only_what_its_gradients_need(launches):
+    """Frozen weights, a bias alone: the pre-activations serve dx, dw_in and db_in, the hidden rows dw_out, and nothing the others."""
+    names = list(FFN)
+    for need, au, h in ((('x',), 1, 0), (('w_in',), 1, 0), (('b_in',), 1, 0), (('w_out',), 0, 1), (('b_out',), 0, 0), (('residual',), 0, 0), (names, 1, 1)):
+        launches.clear()
+        given = {n: t.clone().requires_grad_(n in need) for n, t in FFN.items()}
+        y = block.gated_feed_forward(**given)
+        (name, args), = launches
+        assert name == 'nd_gated_ffn' and (args[11] != 0) == bool(au)
+        saved = y.grad_fn.saved_tensors
+        assert (saved[3] is not None) == bool(h) and (saved[4] is not None) == bool(au)
+        grads = torch.autograd.grad(y, [given[n] for n in need], torch.ones_like(y))
+        assert all(g.shape == given[n].shape for g, n in zip(grads, need))
+        assert len(launches) == (1 if need == ('residual',) else 2)

@@ -535,3 +535,50 @@ def test_gradients_past_a_sequences_end_are_zero_whatever_the_queries_hold(B, T,
         assert within(dq[:1, rest], want[0][0][:, rest], want[0][1][:, rest], dtype)
         for a, b in zip((dq, dk, dv), good):
             assert torch.equal(a[1:], b[1:])
+
+
+# ----------------------------------------------------------------------------------------------------------- partial gradients
+def subsets(names):
+    """Each argument alone, all but each, and the weights or the activations frozen."""
+    return [[n] for n in names] + [[m for m in names if m != n] for n in names] + [[n for n in names if 'w' in n or 'b' in n], names[:1] + names[-1:]]
+
+
+def check_subsets(fn, tensors, dout):
+    """Gradients of some arguments are those of the call in which all require one, to the bit."""
+    names = list(tensors)
+
+    def grads(need):
+        leaves = {n: t.detach().clone().requires_grad_(n in need) for n, t in tensors.items()}
+        out = outputs(fn(**leaves))
+        return dict(zip(need, torch.autograd.grad(out, [leaves[n] for n in need], dout)))
+
+    whole = grads(names)
+    for need in subsets(names):
+        if need:
+            for n, g in grads(need).items():
+                assert torch.equal(g, whole[n]), (need, n)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('M,C,F', [(3, 72, 136), (300, 136, 264), (2100, 264, 680)])
+def test_some_gradients_of_the_feed_forward(M, C, F, dtype):
+    t = dict(x=rnd(M, C, seed=1, dtype=dtype), w_in=rnd(2 * F, C, seed=2, dtype=dtype, scale=C ** -0.5), w_out=rnd(C, F, seed=3, dtype=dtype, scale=F ** -0.5),
+             b_in=rnd(2 * F, seed=4, dtype=dtype, scale=0.3), b_out=rnd(C, seed=5, dtype=dtype, scale=0.3), residual=rnd(M, C, seed=6, dtype=dtype))
+    dy = rnd(M, C, seed=9, dtype=dtype)
+    check_subsets(lambda **a: block.gated_feed_forward(**a, activation='gelu'), t, [dy])
+    t.pop('b_in')                                              # one bias of the two
+    check_subsets(block.gated_feed_forward, t, [dy])
+    t.pop('b_out')
+    check_subsets(block.gated_feed_forward, t, [dy])
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('D,Dv', [(32, 64), (64, 128), (128, 256)])
+def test_some_gradients_of_the_attention_and_the_norm(D, Dv, dtype):
+    B, T, H = 2, 90, 2
+    t = dict(q=rnd(B, T, H, 2 * D, seed=1, dtype=dtype), k=rnd(B, T, 1, 2 * D, seed=2, dtype=dtype), v=rnd(B, T, 1, Dv, seed=3, dtype=dtype))
+    t.update({n: rnd(D, seed=4 + i, dtype=dtype, scale=0.2) for i, n in enumerate(block._LAMBDAS)})
+    check_subsets(lambda **a: block.differential_attention(**a, causal=True), t, [rnd(B, T, H, Dv, seed=9, dtype=dtype)])
+    cos, sin = block.rotary_table(torch.arange(T, device=DEV), D)
+    t = dict(q=t['q'], k=t['k'], q_weight=rnd(2 * D, seed=8, dtype=dtype), k_weight=rnd(2 * D, seed=10, dtype=dtype))
+    check_subsets(lambda **a: block.qk_norm_rope(**a, cos=cos, sin=sin), t, [rnd(B, T, H, 2 * D, seed=11, dtype=dtype), rnd(B, T, 1, 2 * D, seed=12, dtype=dtype)])
