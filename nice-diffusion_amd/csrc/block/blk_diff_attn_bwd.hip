@@ -66,7 +66,7 @@ __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
 // DK, DV: which gradients this launch makes.  Wide heads take two launches: the outputs and operands of both do not fit the registers
 template <typename T, int HD, int NW, bool DK, bool DVG>
-__global__ void __launch_bounds__(64 * NW, (HD * (int)sizeof(T) == 64 ? 3 : (HD * (int)sizeof(T) == 128 ? 2 : 1))) diff_dkv_kernel(const DiffBwdArgs p) {
+__global__ void __launch_bounds__(64 * NW, (HD * (int)sizeof(T) == 64 ? 3 : (NW == 8 ? 2 : 1))) diff_dkv_kernel(const DiffBwdArgs p) {
     using S = DiffBwdShape<T, HD>;
     using TR = Tile<T, S::RB>;
     constexpr int RT = S::RT, STAT = 4 * 64 * 4, STAGE = 2 * RT * S::RB + STAT;     // q rows, dO rows, [lse1, lse2, D1, D2][64]
@@ -550,7 +550,9 @@ struct DiffBwdPlan {
 
 // Rows of 256 bytes (D 33 .. 64 in bf16, to 32 in fp32): 8 waves share the rows that pass by, two to a SIMD in one workgroup a CU,
 // where that still fills the chip (8 x 2048^2 x 8 heads: 390 us for 440 with 4); others 4.  Loops divided as diff_parts says and
-// joined in order.
+// joined in order.  Key kernel: a CU holds three workgroups of 128-byte rows, one of longer ones (134 KB of LDS, with 4 waves too:
+// counting two of those divides one drawn shape in 13 otherwise, and 24 such shapes took 1.5 to 2 % longer).  Query kernel: two, one
+// from 512-byte rows on; three of 128-byte rows would fit, but counting them chose no better (24 shapes: 0.3 % longer).
 static DiffBwdPlan diff_bwd_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int es, int causal) {
     DiffBwdPlan pl{};
     const int g = H / Hk;
@@ -560,7 +562,7 @@ static DiffBwdPlan diff_bwd_plan(int B, int Tq, int Tk, int H, int Hk, int D, in
     // a tile of rows (all heads of the group pass by) in the key kernel, 64 keys in the query kernel, in cycles per row / key
     const int hd = diff_head_dim(D, Dv), rt = hd * es <= 64 * 2 ? 64 : 32;
     int64_t share;
-    pl.row_splits = diff_parts(units * pl.key_blocks, 256 * (hd * es == 64 ? 3 : (hd * es == 128 && pl.waves == 4 ? 2 : 1)), (int64_t)g * ((Tq + rt - 1) / rt), 1,
+    pl.row_splits = diff_parts(units * pl.key_blocks, 256 * (hd * es == 64 ? 3 : 1), (int64_t)g * ((Tq + rt - 1) / rt), 1,
                                rt * (pl.waves / 4) * (es == 4 ? 12.0 : 2.0) * hd, (double)krows * (2 * D + Dv) * 4, causal, share);
     pl.key_splits = diff_parts(units * (((int64_t)Tq * g + 127) / 128), hd * es >= 256 ? 256 : 512, Tk, 64, (es == 4 ? 8.0 : 1.3) * hd, (double)rows * 2 * D * 4, causal, share);
     pl.chunk = (int)share;

@@ -267,3 +267,12 @@ def test_every_accepted_row_count_has_a_tile_that_fits_a_launch(M, C, F):
     for dtype in (_hip.DT_BF16, _hip.DT_F32):
         assert lib.nd_gated_ffn(*ffn_args(M=M, C=C, F=F, ldx=C, ldy=C, dtype=dtype)) == -2, lib.nd_block_last_error()
         assert lib.nd_gated_ffn_bwd_workspace_floats(M, C, F, dtype) > 0
+
+
+def test_the_key_kernels_rows_are_divided_for_the_workgroups_that_fit():
+    """256-byte rows: one workgroup a CU.  192 of them, 16096 rows each: four parts are three full rounds of the chip, eight only more
+    partials (measured 1071 us for 1108)."""
+    lib, (B, T, H, Hk, D, Dv) = _hip.load_block(), (6, 4024, 4, 1, 64, 128)
+    rows_part, keys_part = B * T * Hk * (2 * D + Dv), B * T * H * 2 * D      # floats of one part of dk | dv, and of dq
+    small = 2 * B * T * H + (1 << 16)                          # row statistics, shares of lambda's gradient
+    assert lib.nd_diff_attention_bwd_workspace_floats(B, T, T, H, Hk, D, Dv, _hip.DT_BF16) <= 4 * rows_part + 2 * keys_part + small
