@@ -453,3 +453,28 @@ def test_differential_attention_rows_that_repeat_in_memory():
             got.append((o, *torch.autograd.grad(o, leaves, d)))
         for a, b in zip(*got):
             assert torch.equal(a, b)
+
+
+def test_qk_norm_rope_reciprocal_root():
+    """Rows (1, t, 0, ..) with exact squares, exact mean and no weight: the first channel is the reciprocal root itself.  One correction of
+    the hardware's (1 ulp) leaves its own rounding, half an ulp, and half that of m r: 3/2 half units."""
+    for D in (4, 64, 512):
+        t = torch.arange(1, 2048, dtype=torch.float64) / 1024
+        x = torch.zeros(1, 2047, 1, D)
+        x[0, :, 0, 0], x[0, :, 0, 1] = 1, t.float()
+        x = x.to(DEV)
+        want = ((1 + t * t) / D) ** -0.5
+        got = block.qk_norm_rope(x, x, eps=0.0)[0][0, :, 0, 0].double().cpu()
+        assert ((got - want).abs() <= 1.5 * half_ulp(F32) * want * (1 + 1e-6)).all(), (D, ((got - want).abs() / want).max().item() / half_ulp(F32))
+        # gradient of the second channel's output 1: -x0 x1 r^3 / D, from r^2 and r, two products and the division by D
+        leaf = x.clone().requires_grad_()
+        o, _ = block.qk_norm_rope(leaf, x, eps=0.0)
+        d = torch.zeros_like(o)
+        d[..., 1] = 1
+        g = torch.autograd.grad(o, leaf, d)[0][0, :, 0, 0].double().cpu()
+        ref = -t * want ** 3 / D
+        assert ((g - ref).abs() <= (3 * 1.5 + 4) * half_ulp(F32) * ref.abs() * (1 + 1e-6)).all(), D
+    big = torch.full((1, 1, 1, 8), 1e25, device=DEV)           # the sum of squares leaves fp32: zeros, as the reciprocal root says
+    assert (block.qk_norm_rope(big, big)[0] == 0).all()
+    z = torch.zeros(1, 1, 1, 8, device=DEV)
+    assert (block.qk_norm_rope(z, z)[0] == 0).all() and torch.isnan(block.qk_norm_rope(z, z, eps=0.0)[0]).all()
