@@ -10,8 +10,10 @@
 // dlam is summed from fp32 P2 and dP, not from the rounded O2: it is one number and may cancel.  Rounding to bf16 besides the
 // outputs: P1 - lam P2, dS1, dS2 as operands, O1 and O2.  A sequence of one key has constant maps: dq and dk are made exactly zero.
 //
-// Measured, bf16, 8 x 2048^2 x 8 heads of 64 + 128, causal: keys 250 us, queries 155 us (0.48 and 0.52 PFLOP/s of
-// matrix operations); what bounds them is what bounds the forward pass, with two exponentials and ~12 vector operations a score.
+// Measured, bf16, 8 x 2048^2 x 8 heads of 64 + 128, causal: keys 230 us, queries (with D1 and D2) 161 us (0.52 and 0.50 PFLOP/s of
+// matrix operations); what bounds them is what bounds the forward pass, with two exponentials and ~12 vector operations a score, and
+// LDS reads that no phase starts under the one before it (phase(), below).  Vector registers spilled: 26 by that key kernel (8 waves),
+// 10 by the one of bf16 D <= 32; fp32 with D > 64: 125 by the query kernel, 15 by the key kernel.
 #include "blk_diff_attn.h"
 
 namespace ndb {

@@ -9,10 +9,11 @@
 //
 // Roundings to bf16 besides the outputs: h (operand of the second product), a and u where a backward pass will want them
 // (they are what it reads instead of repeating the first product: 2/9 of its operations), da and du (operands of two
-// products).  Each is off by half a unit, 2^-8 relative; fp32 calls round nothing.
+// products).  Each is off by half a unit, 2^-8 relative; fp32 calls round nothing to fewer bits.  In either type silu, gelu_tanh and the
+// slope of gelu take the hardware's exponential (its argument rounded to fp32 first) and reciprocal, 1 ulp each.
 //
 // Measured, bf16: 16384 x 1024 x 4096 with gradients 1250 us (0.99 PFLOP/s; six products alone by the library: 1240), 65536 x 384 x
-// 1024 forward 230 us (0.67).  The parts are at the kernels and launch choices below.
+// 1024 forward with gelu 233 us (0.66; 215 replayed on one input).  The parts are at the kernels and launch choices below.
 #include "blk_gemm.h"
 
 namespace ndb {
@@ -278,7 +279,9 @@ __global__ void __launch_bounds__(1024) colsum_join_kernel(const ColSum<T> first
 // turn, straight to registers, UNITS pieces requested at a time (bf16 4, fp32 2: 23 us for 24 at 1 x 1024 x 4096), and are summed
 // in wave order.  Both operands take the channels of a piece in the same order, 16 bytes a lane.  Where columns are few (no more
 // than one workgroup a CU) 8 columns: half of the operand stays empty, but twice the CUs read: 12.8 us for 13.9.
-// The block at C 1024, F 4096, bf16 (25 MB, 4.9 us as a copy): 1 row 12.8 us, the tile kernels 28; 32 rows 21 for 30; 33: tiles.
+// The block at C 1024, F 4096, bf16 (25 MB, 4.9 us as a copy), replayed: 1 row 10.8 us (fp32 21.2), this form / the tiles at 4 rows
+// 11.7 / 15.4, 16 rows 14.3 / 15.7, 32 rows 19.0 / 19.2.  Narrower weights gain up to 32 rows (384 / 1024: 9.3 / 12.7), wider ones lose
+// from 17 on (2048 / 8192 at 32 rows: 41 / 31, fp32 93 / 61).
 // What is left are two launches that each start, read for 2 to 3 us and drain.
 constexpr int FEW_ROWS = 32, FEW_NARROW = 2048;
 
@@ -379,12 +382,12 @@ struct Plan {
     int splits, k_tiles;
 };
 
-// Time of a product in cycles of a CU (2.2 GHz), the constants fitted to 180 products of 20 feed-forward shapes, each timed with every
-// tile and several divisions (the choices then cost 1.2 % over the best ones; 300 x 136 to 65536 x 2048).  A workgroup's stage (128
+// Time of a product in cycles of a CU (2.2 GHz), the constants fitted to 198 products of 33 feed-forward shapes, each timed with every
+// tile and several divisions (profiles/block_products_by_tile.txt: the choices cost 1.6 % on the mean over the best ones).  A workgroup's stage (128
 // bytes of k): bf16 3200 / 1120 / 380 at ti 4 / 2 / 1 (LDS and L2 traffic per operation: 275 GFLOP, 16384 x 1024 x 8192, took
 // 230 / 265 / 484 us), fp32 the matrix units' 1024 ti^2, ti 1 a fifth more.  4 / ti workgroups share a CU; a stage takes ~850 to
 // arrive.  What the epilogue moves (`moved`, bytes) goes at ~5 TB/s, worse where one workgroup has the CU to itself and nothing
-// overlaps it (so does gelu's arithmetic: 65536 x 384 x 1024 forward 228 us with ti 4, 210 with 2): the gate's backward product at 16384 x 4096 x 1024 takes 266 / 214 / 272 us, its forward one 283 / 305 / 418.
+// overlaps it (so does gelu's arithmetic: 65536 x 384 x 1024 forward, replayed, 233 us with ti 4, 215 with 2): the gate's backward product at 16384 x 4096 x 1024 takes 266 / 214 / 272 us, its forward one 283 / 305 / 418.
 static Plan plan_gemm(int64_t M, int64_t N, int64_t K, int es, bool gated, bool gelu, bool may_split, double moved) {
     const int kt = 128 / es;
     const int64_t stages = (K + kt - 1) / kt;

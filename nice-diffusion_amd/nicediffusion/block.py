@@ -11,9 +11,9 @@ Conventions.  Tensors live on an AMD GPU (there is no CPU path: ``NdHipError``) 
 sums, softmax statistics and products are fp32.  Work is queued on the current stream of the tensors' device, nothing
 synchronises, scratch memory comes from torch's allocator, so a call may be captured into a hipGraph.  Wrong shapes or dtypes
 raise ``ValueError`` / ``TypeError`` before anything is launched.  All three are differentiable (once): gradients flow to
-every floating argument except the tables; a forward-mode tangent raises ``NotImplementedError``.  To capture a backward pass,
-do it on leaves that no graph built outside the capture still holds (torch ties a leaf's gradient accumulation to the stream of
-its first graph).
+every floating argument except the tables.  A forward-mode tangent raises ``NotImplementedError``; ``torch.func`` transforms
+(vmap, grad, jvp) are not supported and end in torch's own error.  To capture a backward pass, do it on leaves that no graph
+built outside the capture still holds (torch ties a leaf's gradient accumulation to the stream of its first graph).
 """
 import torch
 import torch.autograd.forward_ad as _fwd
@@ -358,7 +358,8 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
     key_lengths [B] (int32 or int64, on the GPU): keys at or past it take no part, whatever their memory holds, and get zero
     gradients; values are held to 0 .. Tk.  causal: query t sees the keys up to t + length - Tq (the queries are the sequence's
     last); it hides by weights of zero, so a NaN or infinite key or value may spoil rows before it too.  A query that sees no key
-    gives a zero row and no gradient.  Returns [B, Tq, H, Dv], contiguous.  Few query rows (Tq H / Hk <= 32, single tokens) have
+    gives a zero row and no gradient.  This is the difference of the maps alone: a norm of each head's output and a factor
+    (1 - lambda_init), where a model has them, are the caller's.  Returns [B, Tq, H, Dv], contiguous.  Few query rows (Tq H / Hk <= 32, single tokens) have
     a form of their own that divides the keys."""
     if q.dim() != 4 or q.shape[3] % 2:
         raise ValueError('q has shape {}, expected [B, Tq, H, 2 D]'.format(tuple(q.shape)))

@@ -220,3 +220,19 @@ def test_the_feed_forward_holds_only_what_its_gradients_need(launches):
         grads = torch.autograd.grad(y, [given[n] for n in need], torch.ones_like(y))
         assert all(g.shape == given[n].shape for g, n in zip(grads, need))
         assert len(launches) == (1 if need == ('residual',) else 2)
+
+
+# ----------------------------------------------------------------------------------------------------- functional transforms
+@pytest.mark.parametrize('fn,tensors', [(block.qk_norm_rope, QK), (block.differential_attention, DIFF), (block.gated_feed_forward, FFN)])
+def test_functional_transforms_end_in_an_error(monkeypatch, no_device, fn, tensors):
+    """vmap, grad and jvp wrap the tensors, and a wrapper has no memory to launch on: no transform returns a result."""
+    def launched(name, device, *args):
+        raise AssertionError('launched')
+    monkeypatch.setattr(block, '_call', launched)
+    first = next(iter(tensors))
+    rest = {n: t for n, t in tensors.items() if n != first}
+    call = lambda t: (lambda o: (o[0] if isinstance(o, tuple) else o).sum())(fn(**{first: t}, **rest))  # noqa: E731
+    for run in (lambda: torch.func.vmap(call)(torch.stack([tensors[first]] * 2)), lambda: torch.func.grad(call)(tensors[first]),
+                lambda: torch.func.jvp(call, (tensors[first],), (torch.ones_like(tensors[first]),)), lambda: torch.func.vjp(call, tensors[first])[1](torch.ones(()))):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            run()
