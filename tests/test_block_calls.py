@@ -236,3 +236,16 @@ def test_functional_transforms_end_in_an_error(monkeypatch, no_device, fn, tenso
                 lambda: torch.func.jvp(call, (tensors[first],), (torch.ones_like(tensors[first]),)), lambda: torch.func.vjp(call, tensors[first])[1](torch.ones(()))):
         with pytest.raises((RuntimeError, NotImplementedError)):
             run()
+
+
+def test_gradients_of_empty_calls(launches):
+    """No rows: zero gradients of every weight, nothing launched."""
+    q, k = r(2, 0, 3, 16).requires_grad_(), r(2, 0, 1, 16).requires_grad_()
+    w = [r(16).requires_grad_() for _ in range(2)]
+    o = block.qk_norm_rope(q, k, *w, cos=r(0, 8), sin=r(0, 8))
+    g = torch.autograd.grad(o, (q, k, *w), [torch.empty_like(t) for t in o])
+    assert g[0].shape == q.shape and g[1].shape == k.shape and all((t == 0).all() for t in g[2:])
+    given = {n: t.clone().requires_grad_() for n, t in FFN.items() if n not in ('x', 'residual')}
+    x = r(2, 0, 16).requires_grad_()
+    g = torch.autograd.grad(block.gated_feed_forward(x, **given), (x, *given.values()), torch.empty(2, 0, 16))
+    assert g[0].shape == x.shape and all((t == 0).all() for t in g[1:]) and not launches

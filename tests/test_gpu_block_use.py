@@ -582,3 +582,34 @@ def test_some_gradients_of_the_attention_and_the_norm(D, Dv, dtype):
     cos, sin = block.rotary_table(torch.arange(T, device=DEV), D)
     t = dict(q=t['q'], k=t['k'], q_weight=rnd(2 * D, seed=8, dtype=dtype), k_weight=rnd(2 * D, seed=10, dtype=dtype))
     check_subsets(lambda **a: block.qk_norm_rope(**a, cos=cos, sin=sin), t, [rnd(B, T, H, 2 * D, seed=11, dtype=dtype), rnd(B, T, 1, 2 * D, seed=12, dtype=dtype)])
+
+
+@pytest.mark.parametrize('dtype', [torch.int32, torch.int64])
+@pytest.mark.parametrize('Tq,causal', [(1, False), (3, True), (60, True)])
+def test_a_captured_step_follows_its_lengths(Tq, causal, dtype):
+    """A decode step captured once and replayed while the cache fills: lengths, queries and one slot of the cache change in place."""
+    B, H, Hk, D, room = 3, 4, 2, 32, 700
+    q, k, v = rnd(B, Tq, H, 2 * D, seed=1, dtype=BF), rnd(B, room, Hk, 2 * D, seed=2, dtype=BF), rnd(B, room, Hk, 2 * D, seed=3, dtype=BF)
+    lams = [rnd(D, seed=30 + i, dtype=BF, scale=0.2) for i in range(4)]
+    ln = torch.zeros(B, dtype=dtype, device=DEV)
+    call = lambda: block.differential_attention(q, k, v, *lams, key_lengths=ln, causal=causal)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for step, lens in enumerate(((0, 1, 2), (700, 699, 33), (64, 65, 0), (900, -3, 350), (1, 1, 1))):
+        ln.copy_(torch.tensor(lens))
+        q.copy_(rnd(*q.shape, seed=10 + step, dtype=BF))
+        k[:, 5 * step] = rnd(B, Hk, 2 * D, seed=20 + step, dtype=BF)
+        out.fill_(math.nan)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), step
+        held = [min(max(n, 0), room) for n in lens]
+        (ref, err), _ = diff_ref(q.double(), k.double(), v.double(), [t.double() for t in lams], 0.8, D ** -0.5, held, causal, half_ulp(BF))
+        assert within(out, ref, err, BF), step
