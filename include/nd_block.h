@@ -28,8 +28,9 @@ const char* nd_block_last_error(void); /* thread-local message of the last faili
 #define ND_ROPE_INTERLEAVED 1 /* rotated pairs are channels (2i, 2i+1); default: (i, i + R/2) */
 
 /* q [B, T, Hq, D], k [B, T, Hk, D] (Hk may be 0) with element strides (batch, token, head), channels contiguous; an output may be
- * its input itself (same pointer and strides), and overlaps nothing else (refused).  weights [D] or NULL.  cos / sin: fp32 [T][R/2] rows, batch stride
- * table_sb (0 = shared by the batch); the first R channels are rotated (R even, 0 = none).  D even, at most 512. */
+ * its input itself (same pointer and strides), and overlaps nothing else (refused).  weights [D] or NULL.  cos / sin: fp32
+ * [T][R/2] rows, batch stride table_sb (0 = shared by the batch); the first R channels are rotated (R even, 0 = none).  D even, at
+ * most 512. */
 int nd_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
                     const void* q_weight, const void* k_weight, const float* cos, const float* sin, int64_t table_sb, void* q_out,
                     int64_t qo_sb, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh, int B, int T,

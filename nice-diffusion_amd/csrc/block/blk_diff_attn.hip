@@ -11,8 +11,9 @@
 // at the price of a pass over the scores for the statistics: the same matrix operations and twice the exponentials.
 //   prefill    4 waves x 32 rows, tiles of 64 keys (fp32 with D > 64: 32), a ring of two (bf16, D <= 32: three), loads straight to
 //              LDS.  bf16, 8 x 2048^2 x 8 heads of 64 + 128: 227 us (0.91 PFLOP/s of matrix operations), causal 132 (141 with what the
-//              backward pass reads written too); 64 x 1024^2 x 6 heads of 32 + 64: 212 us.  Bound by the SIMD's issue: matrix operations and the softmax's vector operations add up
-//              rather than overlap (a fused multiply-add 2.5 cycles beside them, an exponential 2.8 to 8)
+//              backward pass reads written too); 64 x 1024^2 x 6 heads of 32 + 64: 212 us.  Bound by the SIMD's issue: matrix operations
+//              and the softmax's vector operations add up rather than overlap (a fused multiply-add 2.5 cycles beside them, an
+//              exponential 2.8 to 8)
 //   few rows   (g Tq <= 32: single tokens) a kernel of its own: diff_few_kernel
 //   wide heads (D > 64) 128 value channels a workgroup, the scores made twice when Dv is above that: both maps' outputs and the
 //              queries of 256 channels do not fit the registers (measured: 290 spilled)
@@ -585,7 +586,8 @@ int diff_parts(int64_t units, int slots, int64_t length, int64_t grain, double p
 // Few rows: ~256 workgroups, one for each CU (the case above: 50 us; 512 even out ragged lengths, but a second start and join cost
 // more: 58 us, 1024: 74), no split under two tiles for each wave (4 x 8 heads, 2048 keys: 18 us for 20 with one).  fp32: 118 us for
 // 393 MB there (76 us as a copy).  The form ends at 32 rows of a key head: 4 sequences, 16 heads on 4, 8192 keys, causal, 8 new tokens
-// 22.9 us, 9 tokens 33.9, 128 tokens 97 (24.8 of matrix operations).  Many: a workgroup's 32 keys take its CU ~30 HD cycles, fp32 ~190 HD.
+// 22.9 us, 9 tokens 33.9, 128 tokens 97 (24.8 of matrix operations).  Many: a workgroup's 32 keys take its CU ~30 HD cycles, fp32
+// ~190 HD.
 static DiffPlan diff_plan(int B, int Tq, int Tk, int H, int Hk, int D, int Dv, int es, int causal) {
     const int g = H / Hk, rows = Tq * g, hd = diff_head_dim(D, Dv);
     DiffPlan pl{rows <= 32, 1, Tk};

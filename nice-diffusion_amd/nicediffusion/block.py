@@ -359,8 +359,8 @@ def differential_attention(q, k, v, lambda_q1, lambda_k1, lambda_q2, lambda_k2, 
     gradients; values are held to 0 .. Tk.  causal: query t sees the keys up to t + length - Tq (the queries are the sequence's
     last); it hides by weights of zero, so a NaN or infinite key or value may spoil rows before it too.  A query that sees no key
     gives a zero row and no gradient.  This is the difference of the maps alone: a norm of each head's output and a factor
-    (1 - lambda_init), where a model has them, are the caller's.  Returns [B, Tq, H, Dv], contiguous.  Few query rows (Tq H / Hk <= 32, single tokens) have
-    a form of their own that divides the keys."""
+    (1 - lambda_init), where a model has them, are the caller's.  Returns [B, Tq, H, Dv], contiguous.  Few query rows
+    (Tq H / Hk <= 32, single tokens) have a form of their own that divides the keys."""
     if q.dim() != 4 or q.shape[3] % 2:
         raise ValueError('q has shape {}, expected [B, Tq, H, 2 D]'.format(tuple(q.shape)))
     B, Tq, H, D = q.shape
